@@ -291,7 +291,58 @@ int smx_step_key_addr_gemm_ws(void** out);
 int smx_step_key_addr_norm(void** out);
 int smx_step_key_addr_attention(void** out);
 
+/* ---- decoding from a K/V cache (csrc/kvcache.hip, attention_cached.hip, verify.hip) ----
+ * The cached form of the decoder attention (TF:models/bart/modeling_bart.py:133-257, TF:models/t5/modeling_t5.py:281-369 with
+ * past_key_values) behind SpeechMixEED.generate; the reference's own loops re-run the whole prefix per token (ref:train.py:18-34).
+ * Element formats of a cache: SMX_KV_E4M3 / SMX_KV_INT8 one byte per element and one fp32 scale per (row, head, token), value =
+ * code * scale; SMX_KV_BF16 / SMX_KV_F32 plain values (ks = vs = NULL).  Element (b, h, t, d) of k and of v stands at
+ * b * bs + h * hs + t * ts + d, its scale at b * sbs + h * shs + t.  D: a multiple of 8, at most 256; bases 16-byte aligned, bs / hs / ts
+ * multiples of 8 (of 16 in the 8-bit formats with D = 64 or 128 for the matrix-core kernels; other strides take the general one). */
+enum { SMX_KV_E4M3 = 0, SMX_KV_INT8 = 1, SMX_KV_BF16 = 2, SMX_KV_F32 = 3 };
+typedef struct SmxKVCache {
+    void *k, *v; float *ks, *vs; long long bs, hs, ts, sbs, shs; int B, H, cap, D, fmt, _pad;
+} SmxKVCache;
+/* T rows per batch entry at positions start[b] + t (start NULL: start0 + t).  smx_kv_append quantises k / v [B, T, H, D] (strides in
+ * elements, multiples of 8) into the cache; smx_kv_read writes the cache's values there.  A row whose position is outside 0 .. cap - 1 is
+ * dropped (append) or left as it was (read).  e4m3: scale = the smallest power of two with max|x| / scale <= 448; int8: max|x| / 127;
+ * codes round to nearest even.  A row with an element that is not finite is stored as zeros under a NaN scale and reads back as NaN.
+ * dtype (SMX_F32 / SMX_BF16): the type of k and v. */
+typedef struct SmxKVRowsParams {
+    SmxKVCache c; void *k, *v; const int* start; long long k_bs, k_ts, k_hs, v_bs, v_ts, v_hs; int T, start0;
+} SmxKVRowsParams;
+int smx_kv_append(const SmxKVRowsParams* p, int dtype, hipStream_t stream);
+int smx_kv_read(const SmxKVRowsParams* p, int dtype, hipStream_t stream);
+/* Attention of the last Tq tokens of every row (q, o: [B, Tq, H, D], dtype SMX_F32 / SMX_BF16) over its own cache (klen[b] tokens, the Tq
+ * new ones included; own.k NULL: none) behind an optional prefix cache whose entry g the B / pre.B consecutive rows of group g share
+ * (plen[g] tokens).  H a multiple of the caches' heads: query head h reads head h / (H / Hkv).  Prefix keys are visible to every query; with
+ * `causal` query t sees own keys up to position klen - Tq + t.  Lengths are clamped to 0 .. cap; NULL lengths mean cap.  rel_bias [H, nrel]
+ * adds rel_bias[h, clamp(qpos - kpos, 0, nrel - 1)] to the scaled score (positions count the prefix).  A query without a visible key gives
+ * O = 0, lse = -inf.  ws: smx_attention_cached_ws_bytes bytes of device scratch (16-byte aligned), free to reuse once the launches are done;
+ * two launches that may overlap need one each. */
+typedef struct SmxCachedAttnParams {
+    const void* q; void* o; float* lse; SmxKVCache own, pre; const int *klen, *plen; const float* rel_bias;
+    long long q_bs, q_ts, q_hs, o_bs, o_ts, o_hs; void* ws; long long ws_bytes;
+    int B, Tq, H, causal, nrel; float scale;
+} SmxCachedAttnParams;
+long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* p, int dtype);
+int smx_attention_cached(const SmxCachedAttnParams* p, int dtype, hipStream_t stream);
+/* Verification of n drafted ids per row against the target's probabilities [B, n + 1, V], from given uniforms u [B, n + 1] in [0, 1):
+ * draft i is accepted while u_i * q_i(x_i) < p_i(x_i) (draft = NULL: q_i is 1 at x_i); the next token is drawn with u_n from
+ * max(p_r - q_r, 0) at the first rejected draft r, from p when all are accepted or at an id outside 0 .. V - 1 (a shorter draft).  Drawn index:
+ * the smallest whose running sum exceeds u_n times the total (64-bit sums).  n = 0 is plain sampling.  u = NULL: greedy, accepted while id ==
+ * arg max (lowest index of ties; target may be logits).  n <= 64.  ws: smx_verify_draft_ws_bytes bytes (8-byte aligned). */
+typedef struct SmxVerifyParams {
+    const float *target, *draft, *u; const long long* ids; int* accepted; long long* token; void* ws; long long ws_bytes;
+    long long t_bs, t_ts, d_bs, d_ts, ids_bs, u_bs; int B, n, V, _pad;
+} SmxVerifyParams;
+long long smx_verify_draft_ws_bytes(const SmxVerifyParams* p);
+int smx_verify_draft(const SmxVerifyParams* p, hipStream_t stream);
+
 /* ABI self-description */
+int smx_sizeof_SmxKVCache(void);
+int smx_sizeof_SmxKVRowsParams(void);
+int smx_sizeof_SmxCachedAttnParams(void);
+int smx_sizeof_SmxVerifyParams(void);
 int smx_sizeof_SmxGemmParams(void);
 int smx_sizeof_SmxNormParams(void);
 int smx_sizeof_SmxNormBwdParams(void);

@@ -156,3 +156,33 @@ class AfParams(C.Structure):
 class WsumParams(C.Structure):
     _fields_ = [("h", C.c_void_p * 40), ("w", C.c_void_p), ("out", C.c_void_p), ("dy", C.c_void_p), ("dots", C.c_void_p),
                 ("dw", C.c_void_p), ("sw", C.c_void_p), ("n", C.c_longlong), ("L1", C.c_int)]
+
+
+KV_E4M3, KV_INT8, KV_BF16, KV_F32 = 0, 1, 2, 3
+
+
+class KVCacheDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("ks", C.c_void_p), ("vs", C.c_void_p), ("bs", C.c_longlong),
+                ("hs", C.c_longlong), ("ts", C.c_longlong), ("sbs", C.c_longlong), ("shs", C.c_longlong), ("B", C.c_int),
+                ("H", C.c_int), ("cap", C.c_int), ("D", C.c_int), ("fmt", C.c_int), ("_pad", C.c_int)]
+
+
+class KVRowsParams(C.Structure):
+    _fields_ = [("c", KVCacheDesc), ("k", C.c_void_p), ("v", C.c_void_p), ("start", C.c_void_p), ("k_bs", C.c_longlong),
+                ("k_ts", C.c_longlong), ("k_hs", C.c_longlong), ("v_bs", C.c_longlong), ("v_ts", C.c_longlong),
+                ("v_hs", C.c_longlong), ("T", C.c_int), ("start0", C.c_int)]
+
+
+class CachedAttnParams(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("own", KVCacheDesc), ("pre", KVCacheDesc),
+                ("klen", C.c_void_p), ("plen", C.c_void_p), ("rel_bias", C.c_void_p), ("q_bs", C.c_longlong), ("q_ts", C.c_longlong),
+                ("q_hs", C.c_longlong), ("o_bs", C.c_longlong), ("o_ts", C.c_longlong), ("o_hs", C.c_longlong), ("ws", C.c_void_p),
+                ("ws_bytes", C.c_longlong), ("B", C.c_int), ("Tq", C.c_int), ("H", C.c_int), ("causal", C.c_int), ("nrel", C.c_int),
+                ("scale", C.c_float)]
+
+
+class VerifyParams(C.Structure):
+    _fields_ = [("target", C.c_void_p), ("draft", C.c_void_p), ("u", C.c_void_p), ("ids", C.c_void_p), ("accepted", C.c_void_p),
+                ("token", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_longlong), ("t_bs", C.c_longlong), ("t_ts", C.c_longlong),
+                ("d_bs", C.c_longlong), ("d_ts", C.c_longlong), ("ids_bs", C.c_longlong), ("u_bs", C.c_longlong), ("B", C.c_int),
+                ("n", C.c_int), ("V", C.c_int), ("_pad", C.c_int)]

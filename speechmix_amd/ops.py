@@ -1221,3 +1221,236 @@ def scale_dev(x, scale):
 def dropout(x, out, n, p, seed, dtype):
     """out = x * mask(seed) / (1 - p), mask index = flat element index (same function the fused epilogues use)."""
     L.check(L.lib().smx_dropout(C.c_void_p(_ptr(x)), C.c_void_p(_ptr(out)), C.c_longlong(n), C.c_float(p), C.c_uint(seed), dtype, _stream()), "smx_dropout")
+
+
+# ---- decoding from a K/V cache ---------------------------------------------------------------------------------------
+KV_FORMATS = {"e4m3": L.KV_E4M3, "int8": L.KV_INT8, "bf16": L.KV_BF16, "f32": L.KV_F32}
+_KV_STORE = {"e4m3": (torch.uint8, torch.float8_e4m3fn), "int8": (torch.uint8, torch.int8), "bf16": (torch.bfloat16,), "f32": (torch.float32,)}
+
+
+def _need(ok, msg):
+    if not ok:
+        raise RuntimeError(msg)
+
+
+def _on_device(name, **tensors):
+    """Every tensor on the CURRENT device (launches go to its current stream)."""
+    dev = None
+    for n, t in tensors.items():
+        if t is None:
+            continue
+        _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: {n} must be a GPU tensor (no CPU fallback)")
+        dev = torch._C._cuda_getDevice() if dev is None else dev
+        _need(t.device.index == dev, f"{name}: {n} is on {t.device}, the current device is cuda:{dev}")
+
+
+def _disjoint(t):
+    """No two index tuples of t name the same element (a broadcast or overlapping view cannot be written)."""
+    reach = 0
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= reach:
+            return False
+        reach += stride * (size - 1)
+    return True
+
+
+class KVCache:
+    """K/V rows of `B` batch entries, `H` heads, up to `cap` tokens of `D` elements: k, v [B, H, cap, D] and - in the 8-bit formats
+    "e4m3" / "int8" (codes; uint8 tensors or views of the type itself) - their fp32 scales ks, vs [B, H, cap]; value = code * scale.
+    "bf16" / "f32" hold the values.  Views with other strides are fine as long as D is contiguous (and the tokens of the scales are), k and v
+    have the same strides, and the strides are multiples of 8 elements.  The cache does not know its lengths: the caller passes them."""
+
+    def __init__(self, k, v, ks=None, vs=None, fmt="e4m3"):
+        _need(fmt in KV_FORMATS, f"KVCache: unknown format {fmt!r} (one of {sorted(KV_FORMATS)})")
+        _on_device("KVCache", k=k, v=v, ks=ks, vs=vs)
+        _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype,
+              "KVCache: k and v must be [B, H, cap, D] of one type, with the same strides")
+        _need(k.dtype in _KV_STORE[fmt], f"KVCache: {fmt} rows cannot be held in {k.dtype}")
+        B, H, cap, D = k.shape
+        _need(min(B, H, cap, D) > 0 and D % 8 == 0 and D <= 256, f"KVCache: shape {tuple(k.shape)}: the head width must be a multiple of 8, at most 256")
+        _need(D == 1 or k.stride(3) == 1, "KVCache: the head width must be contiguous")
+        _need(all(s % 8 == 0 for s in k.stride()[:3]) and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0,
+              "KVCache: k and v must be 16-byte aligned, with strides in multiples of 8 elements")
+        _need(_disjoint(k), "KVCache: k and v must not overlap themselves")
+        if fmt in ("e4m3", "int8"):
+            _need(ks is not None and vs is not None, f"KVCache: {fmt} needs the scales ks and vs")
+            _need(ks.shape == (B, H, cap) and vs.shape == ks.shape and ks.dtype == vs.dtype == torch.float32 and ks.stride() == vs.stride()
+                  and (cap == 1 or ks.stride(2) == 1) and _disjoint(ks), "KVCache: ks and vs must be fp32 [B, H, cap] with the same strides, tokens contiguous")
+        else:
+            _need(ks is None and vs is None, f"KVCache: {fmt} has no scales")
+        self.k, self.v, self.ks, self.vs, self.fmt = k, v, ks, vs, fmt
+        self.B, self.H, self.cap, self.D = B, H, cap, D
+
+    @classmethod
+    def empty(cls, B, H, cap, D, fmt, device):
+        """A cache of zeros (scales of one)."""
+        dt = _KV_STORE[fmt][0] if fmt in KV_FORMATS else torch.uint8
+        k = torch.zeros(2, B, H, cap, D, dtype=dt, device=device)
+        s = torch.ones(2, B, H, cap, device=device) if fmt in ("e4m3", "int8") else (None, None)
+        return cls(k[0], k[1], s[0], s[1], fmt)
+
+    def bytes(self):
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.ks, self.vs) if t is not None)
+
+    def desc(self):
+        d = L.KVCacheDesc()
+        d.k, d.v, d.ks, d.vs = _ptr(self.k), _ptr(self.v), _ptr(self.ks), _ptr(self.vs)
+        d.bs, d.hs, d.ts = self.k.stride()[:3]
+        if self.ks is not None:
+            d.sbs, d.shs = self.ks.stride()[:2]
+        d.B, d.H, d.cap, d.D, d.fmt = self.B, self.H, self.cap, self.D, KV_FORMATS[self.fmt]
+        return d
+
+
+def _rows4(name, what, t, shape, written=False):
+    """t as [.., .., heads, D] operand rows: right shape, D contiguous, strides in multiples of 8 elements, 16-byte aligned."""
+    _need(t.shape == shape, f"{name}: {what} must be {tuple(shape)}, got {tuple(t.shape)}")
+    _need(t.dtype in (torch.float32, torch.bfloat16), f"{name}: {what} must be float32 or bfloat16, got {t.dtype}")
+    if t.numel():
+        _need(t.stride(3) == 1 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], shape) if n > 1) and t.data_ptr() % 16 == 0,
+              f"{name}: {what} needs a contiguous head width, strides in multiples of 8 elements and 16-byte alignment")
+        _need(not written or _disjoint(t), f"{name}: {what} must not overlap itself")
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], shape))
+
+
+def _kv_rows(name, cache, start, k, v, written):
+    _on_device(name, k=k, v=v, cache=cache.k)
+    _need(k.dim() == 4 and v.shape == k.shape and k.dtype == v.dtype, f"{name}: k and v must be [B, T, H, D] of one type")
+    T = k.shape[1]
+    shape = torch.Size((cache.B, T, cache.H, cache.D))
+    p = L.KVRowsParams()
+    p.c = cache.desc()
+    p.k_bs, p.k_ts, p.k_hs = _rows4(name, "k", k, shape, written)
+    p.v_bs, p.v_ts, p.v_hs = _rows4(name, "v", v, shape, written)
+    p.T = T
+    if isinstance(start, torch.Tensor):
+        _on_device(name, start=start)
+        _need(start.dtype == torch.int32 and start.shape == (cache.B,) and start.is_contiguous(), f"{name}: start must be int32 [B] (or a number)")
+        p.start = _ptr(start)
+    else:
+        _need(-(1 << 31) <= int(start) < (1 << 31), f"{name}: start {start} is out of range")
+        p.start0 = int(start)
+    if T:
+        p.k, p.v = _ptr(k), _ptr(v)
+    return p, BF16 if k.dtype == torch.bfloat16 else F32
+
+
+def kv_append(cache, k, v, start=0):
+    """k, v [B, T, H, D] (fp32 / bf16, any strides with D contiguous) into the cache at positions start .. start + T - 1 (start: a number, or
+    int32 [B] on the device), quantised to the cache's format.  Rows that fall outside the capacity are dropped."""
+    p, dt = _kv_rows("kv_append", cache, start, k, v, False)
+    if p.T:
+        L.check(L.lib().smx_kv_append(C.byref(p), dt, _stream()), "smx_kv_append")
+
+
+def kv_read(cache, start, k, v):
+    """The cache's values at positions start .. start + T - 1 into k, v [B, T, H, D] (fp32 / bf16).  Rows outside the capacity are left alone."""
+    p, dt = _kv_rows("kv_read", cache, start, k, v, True)
+    if p.T:
+        L.check(L.lib().smx_kv_read(C.byref(p), dt, _stream()), "smx_kv_read")
+
+
+def _lens(name, what, t, n):
+    if t is not None:
+        _on_device(name, **{what: t})
+        _need(t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous(), f"{name}: {what} must be contiguous int32 [{n}]")
+    return _ptr(t)
+
+
+def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel_bias=None, prefix=None, prefix_len=None, want_lse=False):
+    """Attention of the LAST Tq tokens of every row, q [B, Tq, H, D] (fp32 / bf16), over the row's cache (klen int32 [B]: its valid tokens, the
+    new ones included; None: the whole capacity) behind an optional `prefix` cache: entry g of it is shared by the B / prefix.B consecutive
+    rows of group g (prefix_len int32 [groups]) and seen by all their queries.  cache = None: only the prefix.  `causal` orders the new
+    tokens among themselves.  H may be a multiple of the caches' heads.  scale: D ** -0.5 unless given.  rel_bias fp32 [H, n]: bias by the
+    distance query - key, clamped to 0 .. n - 1.  A query that sees no key gives zeros and lse = -inf.
+    -> (out [B, Tq, H, D] of q's type, lse fp32 [B, H, Tq] or None)."""
+    name = "attention_cached"
+    _on_device(name, q=q, out=out, rel_bias=rel_bias, cache=cache.k if cache is not None else None, prefix=prefix.k if prefix is not None else None)
+    main = cache if cache is not None else prefix
+    _need(main is not None, f"{name}: neither a cache nor a prefix")
+    _need(q.dim() == 4 and q.shape[1] > 0 and q.shape[2] > 0, f"{name}: q must be [B, Tq, H, D]")
+    B, Tq, H, D = q.shape
+    _need(D == main.D and H % main.H == 0, f"{name}: q {tuple(q.shape)} does not fit a cache of {main.H} heads of {main.D}")
+    _need(cache is None or cache.B == B, f"{name}: the cache holds {cache.B if cache is not None else 0} rows, q {B}")
+    if prefix is not None:
+        _need(B % prefix.B == 0, f"{name}: {B} rows cannot share {prefix.B} prefixes evenly")
+        _need((prefix.H, prefix.D, prefix.fmt) == (main.H, main.D, main.fmt), f"{name}: cache and prefix differ in heads, head width or format")
+    _need(klen is None or cache is not None, f"{name}: klen without a cache")
+    _need(prefix_len is None or prefix is not None, f"{name}: prefix_len without a prefix")
+    if out is None:
+        out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
+    _need(out.dtype == q.dtype, f"{name}: out must have q's type")
+    p = L.CachedAttnParams()
+    p.q_bs, p.q_ts, p.q_hs = _rows4(name, "q", q, q.shape)
+    p.o_bs, p.o_ts, p.o_hs = _rows4(name, "out", out, q.shape, True)
+    lse = torch.empty(B, H, Tq, device=q.device) if want_lse else None
+    if B == 0:
+        return out, lse
+    p.q, p.o, p.lse = _ptr(q), _ptr(out), _ptr(lse)
+    if cache is not None:
+        p.own = cache.desc()
+        p.klen = _lens(name, "klen", klen, B)
+    if prefix is not None:
+        p.pre = prefix.desc()
+        p.plen = _lens(name, "prefix_len", prefix_len, prefix.B)
+    if rel_bias is not None:
+        _need(rel_bias.dtype == torch.float32 and rel_bias.dim() == 2 and rel_bias.shape[0] == H and rel_bias.shape[1] > 0 and rel_bias.is_contiguous(),
+              f"{name}: rel_bias must be contiguous fp32 [H, n]")
+        p.rel_bias, p.nrel = _ptr(rel_bias), rel_bias.shape[1]
+    p.B, p.Tq, p.H, p.causal = B, Tq, H, int(causal)
+    p.scale = float(D ** -0.5 if scale is None else scale)
+    dt = BF16 if q.dtype == torch.bfloat16 else F32
+    lib = L.lib()
+    lib.smx_attention_cached_ws_bytes.restype = C.c_longlong
+    n = lib.smx_attention_cached_ws_bytes(C.byref(p), dt)
+    L.check(0 if n >= 0 else n, "smx_attention_cached_ws_bytes")
+    # a workspace of its own per call, from the caching allocator: calls on other streams and captured graphs never share one
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    p.ws, p.ws_bytes = _ptr(ws), n
+    L.check(lib.smx_attention_cached(C.byref(p), dt, _stream()), "smx_attention_cached")
+    return out, lse
+
+
+def verify_draft(target, ids, draft=None, uniforms=None):
+    """Check drafted tokens ids int64 [B, n] against the target model's probabilities target fp32 [B, n + 1, V].  Sampled (uniforms fp32
+    [B, n + 1] in [0, 1)): draft i is accepted while u_i q_i(x_i) < p_i(x_i), with the draft model's probabilities `draft` fp32 [B, n, V]
+    (None: the drafts were picked, q_i(x_i) = 1); the token after the accepted ones is drawn with the last uniform from the normalised
+    max(p - q, 0) at a rejected draft, from p behind the last accepted one.  An id outside 0 .. V - 1 ends a row's drafts.  n = 0: plain sampling.
+    Greedy (uniforms = None; target may be logits): accepted while the id is the arg max (lowest index of ties).
+    -> (accepted int32 [B], token int64 [B])."""
+    name = "verify_draft"
+    _on_device(name, target=target, ids=ids, draft=draft, uniforms=uniforms)
+    _need(target.dim() == 3 and target.dtype == torch.float32, f"{name}: target must be fp32 [B, n + 1, V]")
+    B, n, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    _need(n >= 0 and n <= 64 and V > 0 and B <= 65535, f"{name}: target {tuple(target.shape)}: 0 .. 64 drafts, 65 535 rows at most")
+    _need(ids.shape == (B, n) and ids.dtype == torch.int64, f"{name}: ids must be int64 [{B}, {n}]")
+    p = L.VerifyParams()
+
+    def rows(what, t, shape):
+        _need(t.shape == shape and t.dtype == torch.float32, f"{name}: {what} must be fp32 {shape}")
+        _need(t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1, f"{name}: {what} must be contiguous along the last axis")
+        return t.stride()
+    p.t_bs, p.t_ts, _ = rows("target", target, (B, n + 1, V))
+    _need(draft is None or uniforms is not None, f"{name}: draft probabilities without uniforms")
+    if draft is not None:
+        p.d_bs, p.d_ts, _ = rows("draft", draft, (B, n, V))
+    if uniforms is not None:
+        p.u_bs, _ = rows("uniforms", uniforms, (B, n + 1))
+    _need(ids.numel() == 0 or n == 1 or ids.stride(1) == 1, f"{name}: ids must be contiguous along the last axis")
+    p.ids_bs = ids.stride(0)
+    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
+    token = torch.empty(B, dtype=torch.int64, device=target.device)
+    if B == 0:
+        return accepted, token
+    p.target, p.u, p.accepted, p.token = _ptr(target), _ptr(uniforms), _ptr(accepted), _ptr(token)
+    if n:
+        p.ids, p.draft = _ptr(ids), _ptr(draft)
+    p.B, p.n, p.V = B, n, V
+    lib = L.lib()
+    lib.smx_verify_draft_ws_bytes.restype = C.c_longlong
+    nb = lib.smx_verify_draft_ws_bytes(C.byref(p))
+    L.check(0 if nb >= 0 else nb, "smx_verify_draft_ws_bytes")
+    ws = torch.empty(nb, dtype=torch.uint8, device=target.device)
+    p.ws, p.ws_bytes = _ptr(ws), nb
+    L.check(lib.smx_verify_draft(C.byref(p), _stream()), "smx_verify_draft")
+    return accepted, token

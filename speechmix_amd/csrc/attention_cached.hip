@@ -88,26 +88,114 @@ static int ca_check(const SmxCachedAttnParams& p, int dtype) {
     return SMX_OK;
 }
 
+#include "attention_cached_mfma.h"
+
+// ---- host ----
+// The matrix-core kernel takes head widths 64 and 128 and every format but f32, where a 16-byte piece of a key is aligned and the offsets of 64
+// keys fit 31 bits.
+static bool ca_mfma_ok(const SmxCachedAttnParams& p) {
+    const SmxKVCache& m = p.own.k ? p.own : p.pre;
+    if (m.fmt == SMX_KV_F32 || (m.D != 64 && m.D != 128)) return false;
+    for (const SmxKVCache* c : {&p.own, &p.pre})
+        if (c->k) {
+            const int es = kv_es(c->fmt);
+            if (((c->bs | c->hs | c->ts) * es) & 15) return false;
+            if (c->ts < 0 || c->ts * es > (1ll << 24)) return false;
+        }
+    return true;
+}
+static int ca_cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
+// splits of `cap` keys for `base` workgroups: enough of them to fill the chip, none with less than `least` keys
+static int ca_splits(long long base, int cap, int least) {
+    const long long want = ca_cdiv(1024, base), most = ca_cdiv(cap, least);
+    const long long n = want < most ? want : most;
+    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long long& items) {
+    const SmxKVCache& m = p.own.k ? p.own : p.pre;
+    pl.Hkv = m.H;
+    pl.G = p.H / m.H;
+    pl.R = p.pre.k ? p.B / p.pre.B : 1;
+    const long long ro = p.own.k ? (long long)p.Tq * pl.G : 0, rp = p.pre.k ? (long long)pl.R * p.Tq * pl.G : 0, rmax = ro > rp ? ro : rp;
+    const int mt = dtype == SMX_F32 || rmax <= 16 ? 1 : rmax <= 32 ? 2 : 4;
+    pl.mbo = ca_cdiv(ro, 16 * mt);
+    pl.mbp = ca_cdiv(rp, 16 * mt);
+    const long long bo = (long long)pl.mbo * p.own.B * pl.Hkv, bp = (long long)pl.mbp * p.pre.B * pl.Hkv;
+    pl.nso = p.own.k ? ca_splits(bo, p.own.cap, 512) : 0;
+    pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, 512) : 0;
+    pl.items_p = (int)(bp * pl.nsp);
+    items = bp * pl.nsp + bo * pl.nso;
+    pl.join = pl.nso + pl.nsp > 1;
+    return mt;
+}
+
+// bytes of workspace smx_attention_cached needs for these sizes (0: none)
+extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp, int dtype) {
+    if (ca_check(*pp, dtype)) return SMX_EINVAL;
+    if (!ca_mfma_ok(*pp)) return 0;
+    CaPlan pl;
+    long long items;
+    const int mt = ca_plan(*pp, dtype, pl, items);
+    return pl.join ? items * 16 * mt * ((pp->own.k ? pp->own.D : pp->pre.D) + 2) * 4 : 0;
+}
+
 #define CA_SIMPLE(FMT)                                                                                                                \
     do {                                                                                                                              \
         const unsigned n = (unsigned)(((long long)p.B * p.H * p.Tq + 3) / 4);                                                         \
         if (dtype == SMX_BF16) hipLaunchKernelGGL((attn_cached_simple<FMT, bf16_t>), dim3(n), dim3(256), 0, stream, p);               \
         else hipLaunchKernelGGL((attn_cached_simple<FMT, float>), dim3(n), dim3(256), 0, stream, p);                                  \
     } while (0)
-
-// bytes of fp32 workspace smx_attention_cached needs for these sizes (0: none)
-extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp, int dtype) { return ca_check(*pp, dtype) ? SMX_EINVAL : 0; }
+#define CA_MFMA_D(FMT, D)                                                                                                             \
+    do {                                                                                                                              \
+        if (dtype == SMX_F32) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 1, float>), grid, dim3(256), 0, stream, p, pl);            \
+        else if (mt == 1) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 1, bf16_t>), grid, dim3(256), 0, stream, p, pl);               \
+        else if (mt == 2) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 2, bf16_t>), grid, dim3(256), 0, stream, p, pl);               \
+        else hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 4, bf16_t>), grid, dim3(256), 0, stream, p, pl);                            \
+    } while (0)
+#define CA_MFMA(FMT)                           \
+    do {                                       \
+        if (D == 64) CA_MFMA_D(FMT, 64);       \
+        else CA_MFMA_D(FMT, 128);              \
+    } while (0)
 
 extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hipStream_t stream) {
     (void)hipGetLastError();
     const SmxCachedAttnParams p = *pp;
     const int rc = ca_check(p, dtype);
     if (rc) return rc;
-    switch (p.own.k ? p.own.fmt : p.pre.fmt) {
-        case SMX_KV_E4M3: CA_SIMPLE(SMX_KV_E4M3); break;
-        case SMX_KV_INT8: CA_SIMPLE(SMX_KV_INT8); break;
-        case SMX_KV_BF16: CA_SIMPLE(SMX_KV_BF16); break;
-        default: CA_SIMPLE(SMX_KV_F32);
+    const int fmt = p.own.k ? p.own.fmt : p.pre.fmt, D = p.own.k ? p.own.D : p.pre.D;
+    if (ca_mfma_ok(p)) {
+        CaPlan pl;
+        long long items;
+        const int mt = ca_plan(p, dtype, pl, items);
+        if (items > 0x7fffffffll) return SMX_EINVAL;
+        if (pl.join) {
+            const long long rows = items * 16 * mt;
+            if (!p.ws || ((size_t)p.ws & 15) || p.ws_bytes < rows * (D + 2) * 4) return SMX_EINVAL;
+            pl.po = (float*)p.ws;
+            pl.pml = pl.po + rows * D;
+        }
+        const dim3 grid((unsigned)items);
+        if (fmt == SMX_KV_E4M3) CA_MFMA(SMX_KV_E4M3);
+        else if (fmt == SMX_KV_INT8) CA_MFMA(SMX_KV_INT8);
+        else CA_MFMA(SMX_KV_BF16);
+        if (pl.join) {
+            const dim3 jg((unsigned)(((long long)p.B * p.H * p.Tq + 3) / 4));
+            if (D == 64) {
+                if (dtype == SMX_F32) hipLaunchKernelGGL((attn_cached_join<64, float>), jg, dim3(256), 0, stream, p, pl, 16 * mt);
+                else hipLaunchKernelGGL((attn_cached_join<64, bf16_t>), jg, dim3(256), 0, stream, p, pl, 16 * mt);
+            } else {
+                if (dtype == SMX_F32) hipLaunchKernelGGL((attn_cached_join<128, float>), jg, dim3(256), 0, stream, p, pl, 16 * mt);
+                else hipLaunchKernelGGL((attn_cached_join<128, bf16_t>), jg, dim3(256), 0, stream, p, pl, 16 * mt);
+            }
+        }
+    } else {
+        switch (fmt) {
+            case SMX_KV_E4M3: CA_SIMPLE(SMX_KV_E4M3); break;
+            case SMX_KV_INT8: CA_SIMPLE(SMX_KV_INT8); break;
+            case SMX_KV_BF16: CA_SIMPLE(SMX_KV_BF16); break;
+            default: CA_SIMPLE(SMX_KV_F32);
+        }
     }
     SMX_CHECK_LAUNCH();
 }

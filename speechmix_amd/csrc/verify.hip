@@ -14,10 +14,11 @@ struct SmxVerifyParams {
     long long t_bs, t_ts, d_bs, d_ts, ids_bs, u_bs;      // element strides (vocabulary contiguous)
     int B, n, V, _pad;
 };
-#define VF_CHUNK 2048        // weights per workgroup: 256 threads x 8
 #define VF_MAXN 64           // drafts per row: one wave decides them all
+#define VF_WAVES 16          // a workgroup of 1 024 threads per row (or per piece of one)
+#define VF_MAXC 64           // workgroups per row
 
-struct VfRow { const float *p, *q; int r, x; };     // weights of the next token: p - q clamped (q null: p, without index x)
+struct VfRow { const float *p, *q; int r, x; float u; };     // weights of the next token: p - q clamped (q null: p, without index x); its uniform
 
 __device__ __forceinline__ double vf_w(const VfRow& f, int i) {
     const double p = (double)f.p[i];
@@ -28,6 +29,7 @@ __device__ __forceinline__ double vf_w(const VfRow& f, int i) {
 __device__ __forceinline__ VfRow vf_accept(const SmxVerifyParams& p, int b) {
     const int i = threadIdx.x & 63;
     bool acc = false, valid = false;
+    const float u_last = p.u[b * p.u_bs + p.n];        // (asked for here: its latency passes under the others')
     if (i < p.n) {
         const long long x = p.ids[b * p.ids_bs + i];
         valid = x >= 0 && x < p.V;
@@ -39,6 +41,7 @@ __device__ __forceinline__ VfRow vf_accept(const SmxVerifyParams& p, int b) {
     }
     const unsigned long long no = ~__ballot(acc);
     VfRow f;
+    f.u = u_last;
     f.r = no ? min(__ffsll((long long)no) - 1, p.n) : p.n;
     const bool rejected = f.r < p.n && ((__ballot(valid) >> f.r) & 1);
     f.p = p.target + b * p.t_bs + f.r * p.t_ts;
@@ -54,96 +57,165 @@ __device__ __forceinline__ double vf_wave_scan(double v) {             // inclus
     }
     return v;
 }
-// sum of the chunk's weights before this thread's eight (exclusive) and of all of them; sh: 4 doubles
-__device__ __forceinline__ double vf_block_scan(double mine, double* sh, double& total) {
-    const double inc = vf_wave_scan(mine);
+// inclusive sum over the workgroup's threads; sh: VF_WAVES doubles
+__device__ __forceinline__ double vf_block_scan(double v, double* sh) {
+    const double inc = vf_wave_scan(v);
     const int w = threadIdx.x >> 6;
     __syncthreads();
     if ((threadIdx.x & 63) == 63) sh[w] = inc;
     __syncthreads();
-    double base = 0.0;
-    total = 0.0;
-    for (int i = 0; i < 4; ++i) {
-        if (i < w) base += sh[i];
-        total += sh[i];
-    }
-    return base + inc - mine;
+    // (every wave scans the sixteen totals in its lanes: a loop over them is sixteen dependent LDS reads)
+    const double t = vf_wave_scan((threadIdx.x & 63) < VF_WAVES ? sh[threadIdx.x & 63] : 0.0);
+    const double base = __shfl(t, w ? w - 1 : 0, 64);
+    return w ? base + inc : inc;
 }
-__device__ __forceinline__ double vf_chunk8(const VfRow& f, int c, int V, double w[8]) {
-    double s = 0.0;
+struct __attribute__((packed, aligned(4))) VfF4 { float v[4]; };       // (rows of an odd vocabulary start at any multiple of 4 bytes)
+__device__ __forceinline__ void vf_load4(const VfRow& f, int i, int hi, double w[4]) {
+    if (i + 4 <= hi) {
+        const VfF4 p = *reinterpret_cast<const VfF4*>(f.p + i);
+        VfF4 q = {{0.f, 0.f, 0.f, 0.f}};
+        if (f.q) q = *reinterpret_cast<const VfF4*>(f.q + i);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int i = c * VF_CHUNK + threadIdx.x * 8 + e;
-        w[e] = i < V ? vf_w(f, i) : 0.0;
-        s += w[e];
+        for (int e = 0; e < 4; ++e) w[e] = i + e == f.x ? 0.0 : fmax((double)p.v[e] - (double)q.v[e], 0.0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = i + e < hi ? vf_w(f, i + e) : 0.0;
     }
-    return s;
 }
-
-__global__ __launch_bounds__(256) void verify_sums_kernel(SmxVerifyParams p, int nchunk, double* sums) {
-    __shared__ double sh[4];
-    const int c = blockIdx.x, b = blockIdx.y;
-    const VfRow f = vf_accept(p, b);
-    double w[8], total;
-    vf_block_scan(vf_chunk8(f, c, p.V, w), sh, total);
-    if (threadIdx.x == 0) sums[(long long)b * nchunk + c] = total;
+// sum of the weights lo .. hi - 1 by one wave.  Four pieces of each operand on the way: the loads stand before any of their uses, without a
+// branch between them (with a check per load 64 rows of 50 265 took 31 us, now 13).
+template <bool Q>
+__device__ __forceinline__ double vf_wave_sum_(const VfRow& f, int lo, int hi) {
+    const int lane = threadIdx.x & 63;
+    double s = 0.0;
+    int i = lo + 4 * lane;
+    for (; i + 3 * 256 + 4 <= hi; i += 4 * 256) {
+        VfF4 p[4], q[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) p[u] = *reinterpret_cast<const VfF4*>(f.p + i + 256 * u);
+        if (Q)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const VfF4*>(f.q + i + 256 * u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            double w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = Q ? fmax((double)p[u].v[e] - (double)q[u].v[e], 0.0) : (double)fmaxf(p[u].v[e], 0.f);
+                if (!Q && i + 256 * u + e == f.x) w[e] = 0.0;
+            }
+            s += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+    }
+    for (; i < hi; i += 256) {
+        double w[4];
+        vf_load4(f, i, hi, w);
+        s += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    return __shfl(vf_wave_scan(s), 63, 64);
 }
-
-__global__ __launch_bounds__(256) void verify_pick_kernel(SmxVerifyParams p, int nchunk, const double* sums) {
-    __shared__ double sh[4];
-    __shared__ int found, last;
-    const int b = blockIdx.x, tid = threadIdx.x;
-    VfRow f = vf_accept(p, b);
-    double total = 0.0;
-    for (int c = 0; c < nchunk; ++c) total += sums[(long long)b * nchunk + c];
-    const bool none = !(total > 0.0);          // p <= q everywhere (rounding of their normalisation): the target's own weights
-    if (none) {
+__device__ __forceinline__ double vf_wave_sum(const VfRow& f, int lo, int hi) { return f.q ? vf_wave_sum_<true>(f, lo, hi) : vf_wave_sum_<false>(f, lo, hi); }
+struct VfShared { double sh[VF_WAVES], before; int seg, lastseg, found, last; };
+// *first = the lowest lane's a among those with `isa`, *last = the highest lane's z among those with `isz`, over the workgroup (a and z ascend
+// with the lane).  One LDS atomic per wave: a thousand of them on one word took 7 us.
+__device__ __forceinline__ void vf_first_last(bool isa, bool isz, int a, int z, int* first, int* last) {
+    const unsigned long long ma = __ballot(isa), mz = __ballot(isz);
+    const int fa = __shfl(a, ma ? __ffsll((long long)ma) - 1 : 0, 64), lz = __shfl(z, mz ? 63 - __clzll((long long)mz) : 0, 64);
+    if ((threadIdx.x & 63) == 0) {
+        if (ma) atomicMin(first, fa);
+        if (mz) atomicMax(last, lz);
+    }
+}
+// The segments' sums -> accepted, token.  mine: the sum of segment threadIdx.x (0 beyond the last of the S segments of `len` weights).
+__device__ __forceinline__ void vf_pick(const SmxVerifyParams& p, int b, VfRow f, double mine, int S, int len, double* sums, VfShared& m) {
+    const int tid = threadIdx.x, w = tid >> 6;
+    double inc = vf_block_scan(mine, m.sh), total = 0.0;
+    __syncthreads();
+    if (tid == (int)blockDim.x - 1) m.before = inc;
+    __syncthreads();
+    total = m.before;
+    if (!(total > 0.0) && (f.q || f.x >= 0)) {       // p <= q everywhere (rounding of their normalisation): the target's own weights
         f.q = nullptr;
         f.x = -1;
-        total = 0.0;
-        for (int c = 0; c < nchunk; ++c) {
-            double w[8], t;
-            vf_block_scan(vf_chunk8(f, c, p.V, w), sh, t);
-            total += t;
-        }
-    }
-    const double goal = (double)p.u[b * p.u_bs + p.n] * total;
-    if (tid == 0) { found = p.V; last = -1; }
-    __syncthreads();
-    double before = 0.0;
-    for (int c = 0; c < nchunk; ++c) {
-        if (!none) {
-            const double s = sums[(long long)b * nchunk + c];
-            if (before + s <= goal && c + 1 < nchunk) { before += s; continue; }
-        }
-        double w[8], t;
-        double run = before + vf_block_scan(vf_chunk8(f, c, p.V, w), sh, t);
-        for (int e = 0; e < 8; ++e) {
-            const int i = c * VF_CHUNK + tid * 8 + e;
-            run += w[e];
-            if (w[e] > 0.0) {
-                atomicMax(&last, i);
-                if (run > goal) { atomicMin(&found, i); break; }
-            }
+        for (int s = w; s < S; s += VF_WAVES) {
+            const double t = vf_wave_sum(f, min(s * len, p.V), min((s + 1) * len, p.V));
+            if ((tid & 63) == 0) sums[s] = t;
         }
         __syncthreads();
-        if (found < p.V) break;
-        before += t;
+        mine = tid < S ? sums[tid] : 0.0;
+        inc = vf_block_scan(mine, m.sh);
+        __syncthreads();
+        if (tid == (int)blockDim.x - 1) m.before = inc;
+        __syncthreads();
+        total = m.before;
     }
-    if (found == p.V) {                        // u_n * total rounded up to the total: the last index that weighs anything
-        for (int c = nchunk - 1; c >= 0 && last < 0; --c) {
-            double w[8];
-            vf_chunk8(f, c, p.V, w);
-            __syncthreads();
-            for (int e = 0; e < 8; ++e)
-                if (w[e] > 0.0) atomicMax(&last, c * VF_CHUNK + tid * 8 + e);
-            __syncthreads();
+    const double goal = (double)f.u * total;
+    if (tid == 0) {
+        m.seg = 0x7fffffff;
+        m.lastseg = 0;
+        m.found = 0x7fffffff;
+        m.last = 0;
+    }
+    __syncthreads();
+    vf_first_last(mine > 0.0 && inc > goal, mine > 0.0, tid, tid, &m.seg, &m.lastseg);
+    __syncthreads();
+    const int seg = min(m.seg, m.lastseg);           // (u_n * total rounded up to the total: the last segment that weighs anything)
+    if (tid == seg) m.before = inc - mine;
+    __syncthreads();
+    double before = m.before;
+    const int hi = min((seg + 1) * len, p.V);
+    for (int lo = seg * len; lo < hi; lo += 4 * 64 * VF_WAVES) {
+        double x[4];
+        const int i = lo + 4 * tid;
+        if (i < hi) vf_load4(f, i, hi, x);
+        else x[0] = x[1] = x[2] = x[3] = 0.0;
+        const double own = (x[0] + x[1]) + (x[2] + x[3]), in2 = vf_block_scan(own, m.sh);
+        double run = before + (in2 - own);
+        int first = -1, lastw = -1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            run += x[e];
+            if (x[e] > 0.0) {
+                lastw = i + e;
+                if (run > goal && first < 0) first = i + e;
+            }
         }
+        vf_first_last(first >= 0, lastw >= 0, first, lastw, &m.found, &m.last);
+        __syncthreads();
+        if (m.found != 0x7fffffff) break;
+        if (tid == (int)blockDim.x - 1) m.before = before + in2;
+        __syncthreads();
+        before = m.before;
     }
     if (tid == 0) {
         p.accepted[b] = f.r;
-        p.token[b] = found < p.V ? found : max(last, 0);
+        p.token[b] = min(m.found, m.last);           // (nothing above the goal in the segment: its last index with a weight)
     }
+}
+
+// One workgroup per row: accept, sum (a wave per sixteenth of the vocabulary), pick.
+__global__ __launch_bounds__(1024) void verify_row_kernel(SmxVerifyParams p, int len) {
+    __shared__ VfShared m;
+    __shared__ double sums[VF_WAVES];
+    const int b = blockIdx.x, w = threadIdx.x >> 6;
+    const VfRow f = vf_accept(p, b);
+    const double t = vf_wave_sum(f, min(w * len, p.V), min((w + 1) * len, p.V));
+    if ((threadIdx.x & 63) == 0) sums[w] = t;
+    __syncthreads();
+    vf_pick(p, b, f, threadIdx.x < VF_WAVES ? sums[threadIdx.x] : 0.0, VF_WAVES, len, sums, m);
+}
+// Few rows: several workgroups sum one row's segments, a second launch picks.
+__global__ __launch_bounds__(1024) void verify_sums_kernel(SmxVerifyParams p, int len, double* sums) {
+    const int b = blockIdx.y, s = blockIdx.x * VF_WAVES + (threadIdx.x >> 6);
+    const VfRow f = vf_accept(p, b);
+    const double t = vf_wave_sum(f, min(s * len, p.V), min((s + 1) * len, p.V));
+    if ((threadIdx.x & 63) == 0) sums[(long long)b * gridDim.x * VF_WAVES + s] = t;
+}
+__global__ __launch_bounds__(1024) void verify_pick_kernel(SmxVerifyParams p, int S, int len, double* sums) {
+    __shared__ VfShared m;
+    const int b = blockIdx.x;
+    sums += (long long)b * S;
+    vf_pick(p, b, vf_accept(p, b), threadIdx.x < S ? sums[threadIdx.x] : 0.0, S, len, sums, m);
 }
 
 // ---- greedy ----
@@ -156,40 +228,44 @@ __device__ __forceinline__ VfBest vf_wave_best(VfBest a) {
     for (int o = 32; o > 0; o >>= 1) vf_better(a, __shfl_xor(a.v, o, 64), __shfl_xor(a.i, o, 64));
     return a;
 }
-__global__ __launch_bounds__(256) void verify_best_kernel(SmxVerifyParams p, int nchunk, VfBest* best) {
-    __shared__ VfBest sh[4];
-    const int c = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
+__global__ __launch_bounds__(1024) void verify_best_kernel(SmxVerifyParams p, VfBest* best) {
+    __shared__ VfBest sh[VF_WAVES];
+    const int i = blockIdx.x, b = blockIdx.y;
     const float* row = p.target + b * p.t_bs + i * p.t_ts;
-    VfBest a = {-INFINITY, c * VF_CHUNK};
+    VfBest a = {-INFINITY, 0x7fffffff};
+    int j = 4 * threadIdx.x;
+    for (; j + 3 * 4096 + 4 <= p.V; j += 4 * 4096) {
+        VfF4 x[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int j = c * VF_CHUNK + e * 256 + threadIdx.x;
-        if (j < p.V) vf_better(a, row[j], j);
+        for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const VfF4*>(row + j + 4096 * u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (x[u].v[e] > a.v) { a.v = x[u].v[e]; a.i = j + 4096 * u + e; }       // (a thread's indices ascend: the first of equals stays)
     }
+    for (; j < p.V; j += 4096)
+        for (int e = 0; e < 4; ++e)
+            if (j + e < p.V && row[j + e] > a.v) { a.v = row[j + e]; a.i = j + e; }
     a = vf_wave_best(a);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 4; ++w) vf_better(a, sh[w].v, sh[w].i);
-        best[((long long)b * (p.n + 1) + i) * nchunk + c] = a;
+    if (threadIdx.x < 64) {
+        a = threadIdx.x < VF_WAVES ? sh[threadIdx.x] : VfBest{-INFINITY, 0x7fffffff};
+        a = vf_wave_best(a);
+        if (a.i == 0x7fffffff) a.i = 0;               // nothing above -inf
+        if (threadIdx.x == 0) best[(long long)b * (p.n + 1) + i] = a;
     }
 }
-__global__ __launch_bounds__(64) void verify_greedy_kernel(SmxVerifyParams p, int nchunk, const VfBest* best) {
+__global__ __launch_bounds__(64) void verify_greedy_kernel(SmxVerifyParams p, const VfBest* best) {
     const int b = blockIdx.x, lane = threadIdx.x;
-    for (int i = 0; i <= p.n; ++i) {
-        const VfBest* row = best + ((long long)b * (p.n + 1) + i) * nchunk;
-        VfBest a = {-INFINITY, 0};
-        if (lane < nchunk) a = row[lane];
-        for (int c = lane + 64; c < nchunk; c += 64) vf_better(a, row[c].v, row[c].i);
-        if (lane >= nchunk) a.i = 0x7fffffff;
-        a = vf_wave_best(a);
-        if (i == p.n || p.ids[b * p.ids_bs + i] != a.i) {
-            if (lane == 0) {
-                p.accepted[b] = i;
-                p.token[b] = a.i;
-            }
-            return;
-        }
+    best += (long long)b * (p.n + 1);
+    const bool ok = lane < p.n && p.ids[b * p.ids_bs + lane] == best[lane].i;
+    const unsigned long long no = ~__ballot(ok);
+    const int r = no ? min(__ffsll((long long)no) - 1, p.n) : p.n;
+    if (lane == 0) {
+        p.accepted[b] = r;
+        p.token[b] = best[r].i;
     }
 }
 
@@ -197,28 +273,42 @@ static int vf_check(const SmxVerifyParams& p) {
     if (!p.target || !p.accepted || !p.token || p.B <= 0 || p.n < 0 || p.n > VF_MAXN || p.V <= 0) return SMX_EINVAL;
     if (p.n > 0 && !p.ids) return SMX_EINVAL;
     if (p.draft && !p.u) return SMX_EINVAL;
-    if (p.B > 65535 || p.V > 0x7fffffff - VF_CHUNK) return SMX_EINVAL;
+    if (p.B > 65535 || p.V > 0x7fffffff - 65536) return SMX_EINVAL;
     return SMX_OK;
 }
-static int vf_chunks(const SmxVerifyParams& p) { return (p.V + VF_CHUNK - 1) / VF_CHUNK; }
+// Workgroups per row of the sampled form (1: the one-launch kernel)
+static int vf_pieces(const SmxVerifyParams& p) {
+    // A workgroup gets through 50 000 weights in about 7 us beside 7 us of latency (ids, probabilities of the drafts, row, scans); a second
+    // launch costs 6.  250 027 weights: one workgroup 30 us, pieces of 32 768 and up 5 + 6 us.
+    const int most = p.V / (VF_WAVES * 2048), want = 256 / p.B;
+    const int c = most < want ? most : want;
+    return c < 2 ? 1 : c > VF_MAXC ? VF_MAXC : c;
+}
 
 extern "C" long long smx_verify_draft_ws_bytes(const SmxVerifyParams* p) {
     if (vf_check(*p)) return SMX_EINVAL;
-    return 8ll * p->B * vf_chunks(*p) * (p->u ? 1 : p->n + 1);
+    if (!p->u) return 8ll * p->B * (p->n + 1);
+    const int c = vf_pieces(*p);
+    return c == 1 ? 0 : 8ll * p->B * c * VF_WAVES;
 }
 extern "C" int smx_verify_draft(const SmxVerifyParams* pp, hipStream_t stream) {
     (void)hipGetLastError();
     const SmxVerifyParams p = *pp;
     const int rc = vf_check(p);
     if (rc) return rc;
-    if (!p.ws || ((size_t)p.ws & 7) || p.ws_bytes < smx_verify_draft_ws_bytes(pp)) return SMX_EINVAL;
-    const int nc = vf_chunks(p);
+    const long long need = smx_verify_draft_ws_bytes(pp);
+    if (need && (!p.ws || ((size_t)p.ws & 7) || p.ws_bytes < need)) return SMX_EINVAL;
     if (p.u) {
-        hipLaunchKernelGGL(verify_sums_kernel, dim3(nc, p.B), dim3(256), 0, stream, p, nc, (double*)p.ws);
-        hipLaunchKernelGGL(verify_pick_kernel, dim3(p.B), dim3(256), 0, stream, p, nc, (const double*)p.ws);
+        const int c = vf_pieces(p), S = c * VF_WAVES, len = ((p.V + S - 1) / S + 3) & ~3;
+        if (c == 1) {
+            hipLaunchKernelGGL(verify_row_kernel, dim3(p.B), dim3(1024), 0, stream, p, len);
+        } else {
+            hipLaunchKernelGGL(verify_sums_kernel, dim3(c, p.B), dim3(1024), 0, stream, p, len, (double*)p.ws);
+            hipLaunchKernelGGL(verify_pick_kernel, dim3(p.B), dim3(1024), 0, stream, p, S, len, (double*)p.ws);
+        }
     } else {
-        hipLaunchKernelGGL(verify_best_kernel, dim3(nc, p.n + 1, p.B), dim3(256), 0, stream, p, nc, (VfBest*)p.ws);
-        hipLaunchKernelGGL(verify_greedy_kernel, dim3(p.B), dim3(64), 0, stream, p, nc, (const VfBest*)p.ws);
+        hipLaunchKernelGGL(verify_best_kernel, dim3(p.n + 1, p.B), dim3(1024), 0, stream, p, (VfBest*)p.ws);
+        hipLaunchKernelGGL(verify_greedy_kernel, dim3(p.B), dim3(64), 0, stream, p, (const VfBest*)p.ws);
     }
     SMX_CHECK_LAUNCH();
 }

@@ -1224,8 +1224,24 @@ def dropout(x, out, n, p, seed, dtype):
 
 
 # ---- decoding from a K/V cache ---------------------------------------------------------------------------------------
+# A decoding step is a few microseconds of kernel, so the checks must not cost more: what a call's checks and sizes follow from - shapes,
+# strides, types, devices, formats; never addresses or values - is its signature, and a signature that has passed once keeps its filled
+# parameter block.  A call with a known signature sets the pointers, checks their alignment and launches.
 KV_FORMATS = {"e4m3": L.KV_E4M3, "int8": L.KV_INT8, "bf16": L.KV_BF16, "f32": L.KV_F32}
 _KV_STORE = {"e4m3": (torch.uint8, torch.float8_e4m3fn), "int8": (torch.uint8, torch.int8), "bf16": (torch.bfloat16,), "f32": (torch.float32,)}
+_SIGNATURES = {}         # signature -> (parameter block, ...) of the three operators
+_SIGNATURES_MAX = 4096   # (forgotten together beyond that: a program with ever new shapes must not grow)
+
+
+def _remember(sig, val):
+    if len(_SIGNATURES) >= _SIGNATURES_MAX:
+        _SIGNATURES.clear()
+    _SIGNATURES[sig] = val
+    return val
+
+
+def _sig(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 def _need(ok, msg):
@@ -1268,7 +1284,7 @@ class KVCache:
         _need(k.dtype in _KV_STORE[fmt], f"KVCache: {fmt} rows cannot be held in {k.dtype}")
         B, H, cap, D = k.shape
         _need(min(B, H, cap, D) > 0 and D % 8 == 0 and D <= 256, f"KVCache: shape {tuple(k.shape)}: the head width must be a multiple of 8, at most 256")
-        _need(D == 1 or k.stride(3) == 1, "KVCache: the head width must be contiguous")
+        _need(k.stride(3) == 1, "KVCache: the head width must be contiguous")
         _need(all(s % 8 == 0 for s in k.stride()[:3]) and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0,
               "KVCache: k and v must be 16-byte aligned, with strides in multiples of 8 elements")
         _need(_disjoint(k), "KVCache: k and v must not overlap themselves")
@@ -1280,6 +1296,13 @@ class KVCache:
             _need(ks is None and vs is None, f"KVCache: {fmt} has no scales")
         self.k, self.v, self.ks, self.vs, self.fmt = k, v, ks, vs, fmt
         self.B, self.H, self.cap, self.D = B, H, cap, D
+        d = self.desc = L.KVCacheDesc()
+        d.k, d.v, d.ks, d.vs = _ptr(k), _ptr(v), _ptr(ks), _ptr(vs)
+        d.bs, d.hs, d.ts = k.stride()[:3]
+        if ks is not None:
+            d.sbs, d.shs = ks.stride()[:2]
+        d.B, d.H, d.cap, d.D, d.fmt = B, H, cap, D, KV_FORMATS[fmt]
+        self.signature = (fmt, k.shape, k.stride(), ks.stride() if ks is not None else None, k.get_device())
 
     @classmethod
     def empty(cls, B, H, cap, D, fmt, device):
@@ -1292,69 +1315,108 @@ class KVCache:
     def bytes(self):
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.ks, self.vs) if t is not None)
 
-    def desc(self):
-        d = L.KVCacheDesc()
-        d.k, d.v, d.ks, d.vs = _ptr(self.k), _ptr(self.v), _ptr(self.ks), _ptr(self.vs)
-        d.bs, d.hs, d.ts = self.k.stride()[:3]
-        if self.ks is not None:
-            d.sbs, d.shs = self.ks.stride()[:2]
-        d.B, d.H, d.cap, d.D, d.fmt = self.B, self.H, self.cap, self.D, KV_FORMATS[self.fmt]
-        return d
-
 
 def _rows4(name, what, t, shape, written=False):
-    """t as [.., .., heads, D] operand rows: right shape, D contiguous, strides in multiples of 8 elements, 16-byte aligned."""
+    """t as [.., .., heads, D] operand rows: right shape, D contiguous, strides in multiples of 8 elements (alignment: at the call)."""
     _need(t.shape == shape, f"{name}: {what} must be {tuple(shape)}, got {tuple(t.shape)}")
     _need(t.dtype in (torch.float32, torch.bfloat16), f"{name}: {what} must be float32 or bfloat16, got {t.dtype}")
     if t.numel():
-        _need(t.stride(3) == 1 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], shape) if n > 1) and t.data_ptr() % 16 == 0,
-              f"{name}: {what} needs a contiguous head width, strides in multiples of 8 elements and 16-byte alignment")
+        _need(t.stride(3) == 1 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], shape) if n > 1),
+              f"{name}: {what} needs a contiguous head width and strides in multiples of 8 elements")
         _need(not written or _disjoint(t), f"{name}: {what} must not overlap itself")
     return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], shape))
 
 
 def _kv_rows(name, cache, start, k, v, written):
-    _on_device(name, k=k, v=v, cache=cache.k)
-    _need(k.dim() == 4 and v.shape == k.shape and k.dtype == v.dtype, f"{name}: k and v must be [B, T, H, D] of one type")
-    T = k.shape[1]
-    shape = torch.Size((cache.B, T, cache.H, cache.D))
-    p = L.KVRowsParams()
-    p.c = cache.desc()
-    p.k_bs, p.k_ts, p.k_hs = _rows4(name, "k", k, shape, written)
-    p.v_bs, p.v_ts, p.v_hs = _rows4(name, "v", v, shape, written)
-    p.T = T
-    if isinstance(start, torch.Tensor):
-        _on_device(name, start=start)
-        _need(start.dtype == torch.int32 and start.shape == (cache.B,) and start.is_contiguous(), f"{name}: start must be int32 [B] (or a number)")
-        p.start = _ptr(start)
+    """The parameter block of kv_append / kv_read -> (block, dtype), or None when there are no rows."""
+    tensor_start = isinstance(start, torch.Tensor)
+    sig = (written, cache.signature, torch._C._cuda_getDevice(), _sig(k), _sig(v), _sig(start) if tensor_start else None)
+    hit = _SIGNATURES.get(sig)
+    if hit is None:
+        _on_device(name, k=k, v=v, cache=cache.k, start=start if tensor_start else None)
+        _need(k.dim() == 4 and v.shape == k.shape and k.dtype == v.dtype, f"{name}: k and v must be [B, T, H, D] of one type")
+        shape = torch.Size((cache.B, k.shape[1], cache.H, cache.D))
+        p = L.KVRowsParams()
+        p.k_bs, p.k_ts, p.k_hs = _rows4(name, "k", k, shape, written)
+        p.v_bs, p.v_ts, p.v_hs = _rows4(name, "v", v, shape, written)
+        p.T = k.shape[1]
+        _need(not tensor_start or (start.dtype == torch.int32 and start.shape == (cache.B,) and start.is_contiguous()),
+              f"{name}: start must be int32 [B] (or a number)")
+        hit = _remember(sig, (bytes(p), BF16 if k.dtype == torch.bfloat16 else F32, p.T))
+    tmpl, dt, T = hit
+    if T == 0:
+        return None
+    p = L.KVRowsParams.from_buffer_copy(tmpl)
+    p.c = cache.desc
+    p.k, p.v = kp, vp = k.data_ptr(), v.data_ptr()
+    if (kp | vp) & 15:
+        raise RuntimeError(f"{name}: k and v must be 16-byte aligned")
+    if tensor_start:
+        p.start = start.data_ptr()
     else:
-        _need(-(1 << 31) <= int(start) < (1 << 31), f"{name}: start {start} is out of range")
+        _need(-(1 << 31) <= int(start) < (1 << 31), f"{name}: a start of {start} is out of range")
         p.start0 = int(start)
-    if T:
-        p.k, p.v = _ptr(k), _ptr(v)
-    return p, BF16 if k.dtype == torch.bfloat16 else F32
+    return p, dt
 
 
 def kv_append(cache, k, v, start=0):
     """k, v [B, T, H, D] (fp32 / bf16, any strides with D contiguous) into the cache at positions start .. start + T - 1 (start: a number, or
     int32 [B] on the device), quantised to the cache's format.  Rows that fall outside the capacity are dropped."""
-    p, dt = _kv_rows("kv_append", cache, start, k, v, False)
-    if p.T:
-        L.check(L.lib().smx_kv_append(C.byref(p), dt, _stream()), "smx_kv_append")
+    r = _kv_rows("kv_append", cache, start, k, v, False)
+    if r:
+        L.check(L.lib().smx_kv_append(C.byref(r[0]), r[1], _stream()), "smx_kv_append")
 
 
 def kv_read(cache, start, k, v):
     """The cache's values at positions start .. start + T - 1 into k, v [B, T, H, D] (fp32 / bf16).  Rows outside the capacity are left alone."""
-    p, dt = _kv_rows("kv_read", cache, start, k, v, True)
-    if p.T:
-        L.check(L.lib().smx_kv_read(C.byref(p), dt, _stream()), "smx_kv_read")
+    r = _kv_rows("kv_read", cache, start, k, v, True)
+    if r:
+        L.check(L.lib().smx_kv_read(C.byref(r[0]), r[1], _stream()), "smx_kv_read")
 
 
-def _lens(name, what, t, n):
-    if t is not None:
-        _on_device(name, **{what: t})
-        _need(t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous(), f"{name}: {what} must be contiguous int32 [{n}]")
-    return _ptr(t)
+def _attention_cached_check(q, cache, klen, out, causal, scale, rel_bias, prefix, prefix_len):
+    """Every check of attention_cached that does not look at an address -> its parameter block, dtype and workspace size."""
+    name = "attention_cached"
+    _on_device(name, q=q, out=out, rel_bias=rel_bias, klen=klen, prefix_len=prefix_len, cache=cache.k if cache is not None else None,
+               prefix=prefix.k if prefix is not None else None)
+    main = cache if cache is not None else prefix
+    _need(main is not None, f"{name}: neither a cache nor a prefix")
+    _need(q.dim() == 4 and q.shape[1] > 0 and q.shape[2] > 0, f"{name}: q must be [B, Tq, H, D]")
+    B, Tq, H, D = q.shape
+    _need(D == main.D and H % main.H == 0, f"{name}: q {tuple(q.shape)} does not fit a cache of {main.H} heads of {main.D}")
+    _need(cache is None or cache.B == B, f"{name}: the cache's rows and q's {B} differ")
+    if prefix is not None:
+        _need(B % prefix.B == 0, f"{name}: {B} rows cannot share {prefix.B} prefixes evenly")
+        _need((prefix.H, prefix.D, prefix.fmt) == (main.H, main.D, main.fmt), f"{name}: cache and prefix differ in heads, head width or format")
+    for what, t, c in (("klen", klen, cache), ("prefix_len", prefix_len, prefix)):
+        if t is not None:
+            _need(c is not None, f"{name}: {what} without its cache")
+            _need(t.dtype == torch.int32 and t.shape == (c.B,) and t.is_contiguous(), f"{name}: {what} must be contiguous int32 [{c.B}]")
+    p = L.CachedAttnParams()
+    p.q_bs, p.q_ts, p.q_hs = _rows4(name, "q", q, q.shape)
+    if out is None:
+        p.o_bs, p.o_ts, p.o_hs = Tq * H * D, H * D, D
+    else:
+        _need(out.dtype == q.dtype, f"{name}: out must have q's type")
+        p.o_bs, p.o_ts, p.o_hs = _rows4(name, "out", out, q.shape, True)
+    if rel_bias is not None:
+        _need(rel_bias.dtype == torch.float32 and rel_bias.dim() == 2 and rel_bias.shape[0] == H and rel_bias.shape[1] > 0 and rel_bias.is_contiguous(),
+              f"{name}: rel_bias must be contiguous fp32 [H, n]")
+        p.nrel = rel_bias.shape[1]
+    p.B, p.Tq, p.H, p.causal = B, Tq, H, int(bool(causal))
+    p.scale = float(D ** -0.5 if scale is None else scale)
+    dt = BF16 if q.dtype == torch.bfloat16 else F32
+    if B == 0:
+        return bytes(p), dt, 0
+    # (the library sizes the workspace from a whole block: the addresses only have to be there)
+    p.own, p.pre = cache.desc if cache is not None else p.own, prefix.desc if prefix is not None else p.pre
+    p.q = p.o = main.desc.k
+    lib = L.lib()
+    lib.smx_attention_cached_ws_bytes.restype = C.c_longlong
+    n = lib.smx_attention_cached_ws_bytes(C.byref(p), dt)
+    L.check(0 if n >= 0 else n, "smx_attention_cached_ws_bytes")
+    p.q = p.o = None
+    return bytes(p), dt, n
 
 
 def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel_bias=None, prefix=None, prefix_len=None, want_lse=False):
@@ -1364,60 +1426,43 @@ def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel
     tokens among themselves.  H may be a multiple of the caches' heads.  scale: D ** -0.5 unless given.  rel_bias fp32 [H, n]: bias by the
     distance query - key, clamped to 0 .. n - 1.  A query that sees no key gives zeros and lse = -inf.
     -> (out [B, Tq, H, D] of q's type, lse fp32 [B, H, Tq] or None)."""
-    name = "attention_cached"
-    _on_device(name, q=q, out=out, rel_bias=rel_bias, cache=cache.k if cache is not None else None, prefix=prefix.k if prefix is not None else None)
-    main = cache if cache is not None else prefix
-    _need(main is not None, f"{name}: neither a cache nor a prefix")
-    _need(q.dim() == 4 and q.shape[1] > 0 and q.shape[2] > 0, f"{name}: q must be [B, Tq, H, D]")
+    sig = (_sig(q), cache.signature if cache is not None else None, prefix.signature if prefix is not None else None, torch._C._cuda_getDevice(),
+           _sig(klen), _sig(prefix_len), _sig(out), _sig(rel_bias), causal, scale)
+    hit = _SIGNATURES.get(sig)
+    if hit is None:
+        hit = _remember(sig, _attention_cached_check(q, cache, klen, out, causal, scale, rel_bias, prefix, prefix_len))
+    tmpl, dt, n = hit
     B, Tq, H, D = q.shape
-    _need(D == main.D and H % main.H == 0, f"{name}: q {tuple(q.shape)} does not fit a cache of {main.H} heads of {main.D}")
-    _need(cache is None or cache.B == B, f"{name}: the cache holds {cache.B if cache is not None else 0} rows, q {B}")
-    if prefix is not None:
-        _need(B % prefix.B == 0, f"{name}: {B} rows cannot share {prefix.B} prefixes evenly")
-        _need((prefix.H, prefix.D, prefix.fmt) == (main.H, main.D, main.fmt), f"{name}: cache and prefix differ in heads, head width or format")
-    _need(klen is None or cache is not None, f"{name}: klen without a cache")
-    _need(prefix_len is None or prefix is not None, f"{name}: prefix_len without a prefix")
     if out is None:
-        out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
-    _need(out.dtype == q.dtype, f"{name}: out must have q's type")
-    p = L.CachedAttnParams()
-    p.q_bs, p.q_ts, p.q_hs = _rows4(name, "q", q, q.shape)
-    p.o_bs, p.o_ts, p.o_hs = _rows4(name, "out", out, q.shape, True)
-    lse = torch.empty(B, H, Tq, device=q.device) if want_lse else None
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Tq), device=q.device) if want_lse else None
     if B == 0:
         return out, lse
-    p.q, p.o, p.lse = _ptr(q), _ptr(out), _ptr(lse)
+    p = L.CachedAttnParams.from_buffer_copy(tmpl)
+    p.q, p.o = qp, op = q.data_ptr(), out.data_ptr()
+    if (qp | op) & 15:
+        raise RuntimeError("attention_cached: q and out must be 16-byte aligned")
+    if lse is not None:
+        p.lse = lse.data_ptr()
     if cache is not None:
-        p.own = cache.desc()
-        p.klen = _lens(name, "klen", klen, B)
+        p.own = cache.desc
+        if klen is not None:
+            p.klen = klen.data_ptr()
     if prefix is not None:
-        p.pre = prefix.desc()
-        p.plen = _lens(name, "prefix_len", prefix_len, prefix.B)
+        p.pre = prefix.desc
+        if prefix_len is not None:
+            p.plen = prefix_len.data_ptr()
     if rel_bias is not None:
-        _need(rel_bias.dtype == torch.float32 and rel_bias.dim() == 2 and rel_bias.shape[0] == H and rel_bias.shape[1] > 0 and rel_bias.is_contiguous(),
-              f"{name}: rel_bias must be contiguous fp32 [H, n]")
-        p.rel_bias, p.nrel = _ptr(rel_bias), rel_bias.shape[1]
-    p.B, p.Tq, p.H, p.causal = B, Tq, H, int(causal)
-    p.scale = float(D ** -0.5 if scale is None else scale)
-    dt = BF16 if q.dtype == torch.bfloat16 else F32
-    lib = L.lib()
-    lib.smx_attention_cached_ws_bytes.restype = C.c_longlong
-    n = lib.smx_attention_cached_ws_bytes(C.byref(p), dt)
-    L.check(0 if n >= 0 else n, "smx_attention_cached_ws_bytes")
-    # a workspace of its own per call, from the caching allocator: calls on other streams and captured graphs never share one
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    p.ws, p.ws_bytes = _ptr(ws), n
-    L.check(lib.smx_attention_cached(C.byref(p), dt, _stream()), "smx_attention_cached")
+        p.rel_bias = rel_bias.data_ptr()
+    if n:
+        # a workspace of its own per call, from the caching allocator: calls on other streams and captured graphs never share one
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        p.ws, p.ws_bytes = ws.data_ptr(), n
+    L.check(L.lib().smx_attention_cached(C.byref(p), dt, _stream()), "smx_attention_cached")
     return out, lse
 
 
-def verify_draft(target, ids, draft=None, uniforms=None):
-    """Check drafted tokens ids int64 [B, n] against the target model's probabilities target fp32 [B, n + 1, V].  Sampled (uniforms fp32
-    [B, n + 1] in [0, 1)): draft i is accepted while u_i q_i(x_i) < p_i(x_i), with the draft model's probabilities `draft` fp32 [B, n, V]
-    (None: the drafts were picked, q_i(x_i) = 1); the token after the accepted ones is drawn with the last uniform from the normalised
-    max(p - q, 0) at a rejected draft, from p behind the last accepted one.  An id outside 0 .. V - 1 ends a row's drafts.  n = 0: plain sampling.
-    Greedy (uniforms = None; target may be logits): accepted while the id is the arg max (lowest index of ties).
-    -> (accepted int32 [B], token int64 [B])."""
+def _verify_check(target, ids, draft, uniforms):
     name = "verify_draft"
     _on_device(name, target=target, ids=ids, draft=draft, uniforms=uniforms)
     _need(target.dim() == 3 and target.dtype == torch.float32, f"{name}: target must be fp32 [B, n + 1, V]")
@@ -1438,19 +1483,47 @@ def verify_draft(target, ids, draft=None, uniforms=None):
         p.u_bs, _ = rows("uniforms", uniforms, (B, n + 1))
     _need(ids.numel() == 0 or n == 1 or ids.stride(1) == 1, f"{name}: ids must be contiguous along the last axis")
     p.ids_bs = ids.stride(0)
-    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
-    token = torch.empty(B, dtype=torch.int64, device=target.device)
-    if B == 0:
-        return accepted, token
-    p.target, p.u, p.accepted, p.token = _ptr(target), _ptr(uniforms), _ptr(accepted), _ptr(token)
-    if n:
-        p.ids, p.draft = _ptr(ids), _ptr(draft)
     p.B, p.n, p.V = B, n, V
+    if B == 0:
+        return bytes(p), 0
+    # (the workspace is sized from a whole block: the addresses only have to be there)
+    p.target = p.accepted = p.token = target.data_ptr()
+    p.u, p.ids = (p.target if uniforms is not None else None), (p.target if n else None)
     lib = L.lib()
     lib.smx_verify_draft_ws_bytes.restype = C.c_longlong
     nb = lib.smx_verify_draft_ws_bytes(C.byref(p))
     L.check(0 if nb >= 0 else nb, "smx_verify_draft_ws_bytes")
-    ws = torch.empty(nb, dtype=torch.uint8, device=target.device)
-    p.ws, p.ws_bytes = _ptr(ws), nb
-    L.check(lib.smx_verify_draft(C.byref(p), _stream()), "smx_verify_draft")
+    p.target = p.accepted = p.token = p.u = p.ids = None
+    return bytes(p), nb
+
+
+def verify_draft(target, ids, draft=None, uniforms=None):
+    """Check drafted tokens ids int64 [B, n] against the target model's probabilities target fp32 [B, n + 1, V].  Sampled (uniforms fp32
+    [B, n + 1] in [0, 1)): draft i is accepted while u_i q_i(x_i) < p_i(x_i), with the draft model's probabilities `draft` fp32 [B, n, V]
+    (None: the drafts were picked, q_i(x_i) = 1); the token after the accepted ones is drawn with the last uniform from the normalised
+    max(p - q, 0) at a rejected draft, from p behind the last accepted one.  An id outside 0 .. V - 1 ends a row's drafts.  n = 0: plain sampling.
+    Greedy (uniforms = None; target may be logits): accepted while the id is the arg max (lowest index of ties).
+    -> (accepted int32 [B], token int64 [B])."""
+    sig = (_sig(target), _sig(ids), _sig(draft), _sig(uniforms), torch._C._cuda_getDevice())
+    hit = _SIGNATURES.get(sig)
+    if hit is None:
+        hit = _remember(sig, _verify_check(target, ids, draft, uniforms))
+    tmpl, n = hit
+    B = target.shape[0]
+    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
+    token = torch.empty(B, dtype=torch.int64, device=target.device)
+    if B == 0:
+        return accepted, token
+    p = L.VerifyParams.from_buffer_copy(tmpl)
+    p.target, p.accepted, p.token = target.data_ptr(), accepted.data_ptr(), token.data_ptr()
+    if ids.shape[1]:
+        p.ids = ids.data_ptr()
+        if draft is not None:
+            p.draft = draft.data_ptr()
+    if uniforms is not None:
+        p.u = uniforms.data_ptr()
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=target.device)
+        p.ws, p.ws_bytes = ws.data_ptr(), n
+    L.check(L.lib().smx_verify_draft(C.byref(p), _stream()), "smx_verify_draft")
     return accepted, token

@@ -539,16 +539,17 @@ class SpeechMixEED(nn.Module):
         lc = self.decoder_model.config
         n = int(max_length if max_length is not None else getattr(lc, "max_length", 20) or 20)
         ids, _ = self.engine.greedy_decode(enc, B, S, n, lc.decoder_start_token_id, lc.eos_token_id, lc.pad_token_id)
+        return self._cut_at_eos(ids)
+
+    def _cut_at_eos(self, ids):
+        lc = self.decoder_model.config
         rows = []
         for r in ids.cpu().tolist():
             rows.append(r[:r.index(lc.eos_token_id)] if lc.eos_token_id in r else r)
         return rows
 
-    @torch.no_grad()
-    def generate(self, input_values, max_length=None):
-        """Greedy transcription: speech encoder, adapters and LM text encoder run ONCE, then a KV-cached decoder step per
-        token (the reference's notebook loop re-runs the whole model per token, ref:eval.ipynb cell 6).  Returns one list of
-        generated token ids per clip (no start token, cut before eos)."""
+    def _speech_encode(self, input_values):
+        """Waveforms -> (LM encoder output [B * S, d], B, S), in eval mode."""
         self._need_engine()
         eng = self.engine
         self.store.refresh_shadow()
@@ -563,23 +564,94 @@ class SpeechMixEED(nn.Module):
             ops.weighted_sum_fwd(hidden, eng.P("weights_sum"), xin, sw, B * T * eng.ec.hidden_size, eng.dt)
             x = xin
         e, S, _ = eng.bridge_fwd(x, B, T)
-        enc = eng.lm_encode(e, None, B, S)
-        return self._greedy(enc, B, S, max_length)
+        return eng.lm_encode(e, None, B, S), B, S
 
-    @torch.no_grad()
-    def generate_from_text(self, input_ids, max_length=None):
-        """LM-only greedy decoding of token ids [B, S] - what `create_self_decoder_input` loops over to make labels
-        (ref:train.py:18-34: decoder_length = max(config.max_length, len(input)); stop at eos)."""
+    def _text_encode(self, ids):
         self._need_engine()
         self.store.refresh_shadow()
-        ids = torch.as_tensor(input_ids).to(self.device)
+        B, S = ids.shape
+        return self.engine.lm_encode(None, ids.to(self.device).reshape(-1).contiguous(), B, S), B, S
+
+    def _decode_options(self, num_return_sequences, do_sample, temperature, kv_cache, assistant_model, num_assistant_tokens, generator):
+        """Checks of generate's options -> True when the plain greedy loop serves them."""
+        from . import decoding
+        decoding.cache_format(kv_cache, self.compute_dtype)
+        if int(num_return_sequences) != num_return_sequences or num_return_sequences < 1:
+            raise ValueError(f"num_return_sequences must be a positive number, got {num_return_sequences!r}")
+        if num_return_sequences > 1 and not do_sample:
+            raise ValueError("num_return_sequences > 1 needs do_sample=True (greedy rows would all be the same)")
+        if not (temperature > 0 and math.isfinite(temperature)):
+            raise ValueError(f"temperature must be positive and finite, got {temperature!r} (do_sample=False is the greedy limit)")
+        if generator is not None and not do_sample:
+            raise ValueError("generator without do_sample=True")
+        if assistant_model is not None:
+            if not isinstance(assistant_model, SpeechMixEED):
+                raise TypeError("assistant_model must be a model of this package")
+            a, t = assistant_model.decoder_model.config, self.decoder_model.config
+            if (a.vocab_size, a.eos_token_id, a.decoder_start_token_id) != (t.vocab_size, t.eos_token_id, t.decoder_start_token_id):
+                raise ValueError("assistant_model must share the vocabulary and its eos / start ids")
+            if not 1 <= num_assistant_tokens <= 64:
+                raise ValueError(f"num_assistant_tokens must be 1 .. 64, got {num_assistant_tokens!r}")
+        return not do_sample and kv_cache is None and assistant_model is None
+
+    def _cached_decode(self, enc, B, S, max_length, num_return_sequences, do_sample, temperature, kv_cache, assistant_model, assistant_enc,
+                       num_assistant_tokens, generator):
+        from . import decoding
+        lc = self.decoder_model.config
+        n = int(max_length if max_length is not None else getattr(lc, "max_length", 20) or 20)
+        inv_t = 1.0 / temperature if do_sample else 1.0
+        nd = num_assistant_tokens if assistant_model is not None else 0
+
+        def decoder(model, enc, S):
+            model.engine._check_positions(Ld=n)
+            return decoding.CachedDecoder(model.engine, enc, B, S, num_return_sequences, n + nd + 1, kv_cache, inv_t)
+        dec = decoder(self, enc, S)
+        draft = None
+        if assistant_model is not None:
+            aenc, aB, aS = assistant_enc
+            assert aB == B
+            draft = decoder(assistant_model, aenc, aS)
+        ids, self.last_decode_steps = decoding.decode(dec, n, lc.decoder_start_token_id, lc.eos_token_id, lc.pad_token_id, sample=do_sample,
+                                                      generator=generator, draft=draft, num_draft=nd)
+        return self._cut_at_eos(ids)
+
+    @torch.no_grad()
+    def generate(self, input_values, max_length=None, *, num_return_sequences=1, do_sample=False, temperature=1.0, kv_cache=None,
+                 assistant_model=None, num_assistant_tokens=4, generator=None):
+        """Transcription: speech encoder, adapters and LM text encoder run ONCE, then a KV-cached decoder step per token (the reference's
+        notebook loop re-runs the whole model per token, ref:eval.ipynb cell 6).  Returns one list of generated token ids per row (no start
+        token, cut before eos): a row per clip, or num_return_sequences consecutive rows per clip.
+
+        Greedy unless do_sample=True (from softmax(logits / temperature), with uniforms of `generator`, a torch.Generator on the model's
+        device).  kv_cache: "fp8" (e4m3 with a power-of-two scale per token and head) or "int8" keeps the decoder's self- and
+        cross-attention keys and values in one byte per element; "bf16" / "fp32" / None in the model's type.  The cross-attention keys of a clip
+        are kept once for all its rows.  assistant_model: a smaller model of the same vocabulary whose decoder drafts num_assistant_tokens
+        tokens at a time for this one to verify - the same tokens (greedy) or the same distribution (sampled) in fewer steps."""
+        args = (num_return_sequences, do_sample, temperature, kv_cache, assistant_model, num_assistant_tokens, generator)
+        plain = self._decode_options(*args)
+        enc, B, S = self._speech_encode(input_values)
+        if plain:
+            return self._greedy(enc, B, S, max_length)
+        aenc = assistant_model._speech_encode(input_values) if assistant_model is not None else None
+        return self._cached_decode(enc, B, S, max_length, *args[:5], aenc, *args[5:])
+
+    @torch.no_grad()
+    def generate_from_text(self, input_ids, max_length=None, *, num_return_sequences=1, do_sample=False, temperature=1.0, kv_cache=None,
+                           assistant_model=None, num_assistant_tokens=4, generator=None):
+        """LM-only decoding of token ids [B, S] - what `create_self_decoder_input` loops over to make labels (ref:train.py:18-34:
+        decoder_length = max(config.max_length, len(input)); stop at eos).  The options are `generate`'s."""
+        args = (num_return_sequences, do_sample, temperature, kv_cache, assistant_model, num_assistant_tokens, generator)
+        plain = self._decode_options(*args)
+        ids = torch.as_tensor(input_ids)
         if ids.dim() == 1:
             ids = ids[None]
-        B, S = ids.shape
-        enc = self.engine.lm_encode(None, ids.reshape(-1).contiguous(), B, S)
+        enc, B, S = self._text_encode(ids)
         if max_length is None:
             max_length = max(int(getattr(self.decoder_model.config, "max_length", 20) or 20), S)
-        return self._greedy(enc, B, S, max_length)
+        if plain:
+            return self._greedy(enc, B, S, max_length)
+        aenc = assistant_model._text_encode(ids) if assistant_model is not None else None
+        return self._cached_decode(enc, B, S, max_length, *args[:5], aenc, *args[5:])
 
     @_builtin
     def cal_loss(self, inputs_embeds=None, attention_mask=None, decoder_input_ids=None, labels=None):

@@ -117,7 +117,7 @@ static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long lon
     pl.G = p.H / m.H;
     pl.R = p.pre.k ? p.B / p.pre.B : 1;
     const long long ro = p.own.k ? (long long)p.Tq * pl.G : 0, rp = p.pre.k ? (long long)pl.R * p.Tq * pl.G : 0, rmax = ro > rp ? ro : rp;
-    const int mt = dtype == SMX_F32 || rmax <= 16 ? 1 : rmax <= 32 ? 2 : 4;
+    const int mt = dtype == SMX_F32 || rmax <= 16 ? 1 : rmax <= 32 || m.D == 128 ? 2 : 4;
     pl.mbo = ca_cdiv(ro, 16 * mt);
     pl.mbp = ca_cdiv(rp, 16 * mt);
     const long long bo = (long long)pl.mbo * p.own.B * pl.Hkv, bp = (long long)pl.mbp * p.pre.B * pl.Hkv;
@@ -150,7 +150,7 @@ extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp
         if (dtype == SMX_F32) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 1, float>), grid, dim3(256), 0, stream, p, pl);            \
         else if (mt == 1) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 1, bf16_t>), grid, dim3(256), 0, stream, p, pl);               \
         else if (mt == 2) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 2, bf16_t>), grid, dim3(256), 0, stream, p, pl);               \
-        else hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 4, bf16_t>), grid, dim3(256), 0, stream, p, pl);                            \
+        else hipLaunchKernelGGL((attn_cached_mfma<FMT, D, D == 64 ? 4 : 2, bf16_t>), grid, dim3(256), 0, stream, p, pl);              \
     } while (0)
 #define CA_MFMA(FMT)                           \
     do {                                       \

@@ -7,15 +7,26 @@
 // as the rounding of the output.
 //   K operand: a lane's 16 contiguous bytes of one key ARE eight k-indices of two (one for bf16) products; Q is loaded in the same order.
 //   V operand: a lane takes DPL = D / 16 neighbouring elements of each of its eight keys; one byte permute per register pairs two keys.
-// Softmax: every wave keeps its own reference m per row and moves it only when a score passes m + 16 (a wave-wide test): probabilities stay
-// below 2^24, and most blocks need no rescaling and no cross-lane maximum.  Four waves take every fourth block of BK keys, and meet in LDS;
+// Softmax in units of log 2: every wave keeps its own reference m per row and moves it only when a score passes m + 16 (a wave-wide test):
+// probabilities stay below 2^16, and most blocks need no rescaling and no cross-lane maximum.  Four waves take every fourth block of BK keys, and meet in LDS;
 // long caches are split over workgroups as well, whose unnormalised (m, l, O) a second kernel joins in a fixed order.
 #pragma once
 #include "kv_common.h"
 
 #define CA_WAVES 4
+#ifndef CA_OCC
+#define CA_OCC 4
+#endif
+#ifndef CA_NB2
+#define CA_NB2 0
+#endif
 #define CA_LOG2E 1.44269504088896340736f
-#define CA_SLACK 16.f             // a score may pass the reference by this much (natural units) before it moves
+#define CA_LN2 0.69314718055994530942f
+#define CA_SLACK 16.f             // a score may pass the reference by this much (log 2 units) before it moves
+#define CA_LOWEST (-3.402823466e38f)
+
+// waves per SIMD the registers are held to
+constexpr int ca_occ(int es, int d, int mt, int qsize) { return qsize == 4 || (es == 2 && d == 128) || mt > 2 || (mt == 2 && d == 128) ? 2 : mt == 2 || d == 128 ? 3 : CA_OCC; }
 
 struct CaPlan {
     int G, Hkv, R;                // query heads per KV head; rows per prefix
@@ -30,8 +41,6 @@ template <int FMT> struct CaFmt;
 template <> struct CaFmt<SMX_KV_E4M3> { enum { ES = 1 }; };
 template <> struct CaFmt<SMX_KV_INT8> { enum { ES = 1 }; };
 template <> struct CaFmt<SMX_KV_BF16> { enum { ES = 2 }; };
-
-struct __attribute__((packed, aligned(4))) CaF4 { float v[4]; };
 
 __device__ __forceinline__ f32x4_t ca_mfma(const unsigned a[4], const unsigned b[4], f32x4_t c) {
     union { unsigned u[4]; bf16x8_t v; } x, y;
@@ -53,74 +62,103 @@ __device__ __forceinline__ void ca_cvt4(unsigned u, unsigned& lo, unsigned& hi) 
         hi = pack_bf2((float)(signed char)(u >> 16), (float)(signed char)(u >> 24));
     }
 }
-__device__ __forceinline__ float ca_exp(float x) { return __builtin_amdgcn_exp2f(x * CA_LOG2E); }
+__device__ __forceinline__ float ca_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// log-sum-exp in natural units from a reference in log 2 units (a bias of the type's lowest value stays what it is)
+__device__ __forceinline__ float ca_lse(float m, float l) {
+    return l == 0.f ? -INFINITY : m == CA_LOWEST ? CA_LOWEST : fmaf(m, CA_LN2, logf(l));
+}
 
-// one wave's block of BK keys in flight
+typedef __attribute__((ext_vector_type(4))) unsigned ca_u4;
+typedef __attribute__((ext_vector_type(2))) unsigned ca_u2;
+// One wave's block of BK keys in flight.  K (with its scales) is asked for again as soon as the scores are out, V as soon as the second product is:
+// each is on its way while the other is worked on, out of one set of registers.  All loads go through buffer descriptors that end behind the
+// last visible key: what lies past it comes back as zeros, and there is one code path for whole and partial blocks.
 template <int FMT, int D, int NB>
 struct CaBlock {
     enum { ES = CaFmt<FMT>::ES, KC = D * ES / 64, VW = D * ES / 64 };      // 16-byte K chunks, V registers per key
-    uint4 k[2 * NB][KC];
+    ca_u4 k[2 * NB][KC];
     unsigned v[2 * NB][4][VW];
-    CaF4 ks[2 * NB], vs[2 * NB];
+    unsigned ks, vs;        // lane (g, i): the scale of key 16 (i >> 2) + 4 g + (i & 3); DPP row broadcasts hand it to the other lanes of g
 };
-
-template <int FMT, int D, int NB, bool TAIL>
-__device__ __forceinline__ void ca_load(CaBlock<FMT, D, NB>& x, const SmxKVCache& c, long long base, long long sbase, int j0, int nmax) {
-    typedef CaBlock<FMT, D, NB> B;
+struct CaView {             // one head of a cache
+    const char *k, *v;
+    const float *ks, *vs;
+    int tsb;                // bytes between tokens
+    int nmax;
+};
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t ca_rsrc(const void* base, long long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)(bytes < 0x7ffffff0ll ? bytes : 0x7ffffff0ll), 0x00020000);
+}
+template <int FMT, int D, int NB>
+__device__ __forceinline__ unsigned ca_load_scales(const float* s, const CaView& c, int j0) {
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const char* kb = (const char*)c.k + (base + (long long)j0 * c.ts) * B::ES;
-    const char* vb = (const char*)c.v + (base + (long long)j0 * c.ts) * B::ES;
-    const int tsb = (int)c.ts * B::ES, last = nmax - 1 - j0;       // (TAIL: keys past the last visible one read the last one)
+    return __builtin_amdgcn_raw_buffer_load_b32(ca_rsrc(s + j0, (c.nmax - j0) * 4ll), 4 * (16 * (i >> 2) + 4 * g + (i & 3)), 0, 0);
+}
+template <int FMT, int D, int NB>
+__device__ __forceinline__ void ca_load_k(CaBlock<FMT, D, NB>& x, const CaView& c, int j0) {
+    typedef CaBlock<FMT, D, NB> B;
+    const int lane = threadIdx.x & 63, off = (lane & 15) * c.tsb + 16 * (lane >> 4);
+    const __amdgpu_buffer_rsrc_t rs = ca_rsrc(c.k + (long long)j0 * c.tsb, (long long)(c.nmax - 1 - j0) * c.tsb + D * B::ES);
+    if (FMT <= SMX_KV_INT8) x.ks = ca_load_scales<FMT, D, NB>(c.ks, c, j0);
 #pragma unroll
-    for (int a = 0; a < 2 * NB; ++a) {
-        const int tk = TAIL ? min(16 * a + i, last) : i;
-        const char* p = kb + (TAIL ? 0ll : 16ll * a * tsb);
-        const unsigned off = (unsigned)(tk * tsb + 16 * g);
+    for (int a = 0; a < 2 * NB; ++a)
 #pragma unroll
-        for (int q = 0; q < B::KC; ++q) x.k[a][q] = *reinterpret_cast<const uint4*>(p + off + 64 * q);
-    }
+        for (int q = 0; q < B::KC; ++q) x.k[a][q] = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16 * a * c.tsb + 64 * q, 0, 0);
+}
+template <int FMT, int D, int NB>
+__device__ __forceinline__ void ca_load_v(CaBlock<FMT, D, NB>& x, const CaView& c, int j0) {
+    typedef CaBlock<FMT, D, NB> B;
+    const int lane = threadIdx.x & 63, off = 4 * (lane >> 4) * c.tsb + 4 * B::VW * (lane & 15);
+    const __amdgpu_buffer_rsrc_t rs = ca_rsrc(c.v + (long long)j0 * c.tsb, (long long)(c.nmax - 1 - j0) * c.tsb + D * B::ES);
+    if (FMT <= SMX_KV_INT8) x.vs = ca_load_scales<FMT, D, NB>(c.vs, c, j0);
 #pragma unroll
     for (int a = 0; a < 2 * NB; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int tk = TAIL ? min(16 * a + 4 * g + r, last) : 4 * g;
-            const char* p = vb + (TAIL ? 0ll : (16ll * a + r) * tsb);
-            const unsigned off = (unsigned)(tk * tsb + 4 * B::VW * i);
-            if (B::VW == 1) x.v[a][r][0] = *reinterpret_cast<const unsigned*>(p + off);
+            const int o = off + (16 * a + r) * c.tsb;
+            if (B::VW == 1) x.v[a][r][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, o, 0, 0);
             else if (B::VW == 2) {
-                const uint2 u = *reinterpret_cast<const uint2*>(p + off);
-                x.v[a][r][0] = u.x;
-                x.v[a][r][B::VW > 1 ? 1 : 0] = u.y;
+                const ca_u2 u = __builtin_amdgcn_raw_buffer_load_b64(rs, o, 0, 0);
+                x.v[a][r][0] = u[0];
+                x.v[a][r][B::VW > 1 ? 1 : 0] = u[1];
             } else {
-                const uint4 u = *reinterpret_cast<const uint4*>(p + off);
-                x.v[a][r][0] = u.x;
-                x.v[a][r][B::VW > 1 ? 1 : 0] = u.y;
-                x.v[a][r][B::VW > 2 ? 2 : 0] = u.z;
-                x.v[a][r][B::VW > 2 ? 3 : 0] = u.w;
+                const ca_u4 u = __builtin_amdgcn_raw_buffer_load_b128(rs, o, 0, 0);
+                x.v[a][r][0] = u[0];
+                x.v[a][r][B::VW > 1 ? 1 : 0] = u[1];
+                x.v[a][r][B::VW > 2 ? 2 : 0] = u[2];
+                x.v[a][r][B::VW > 2 ? 3 : 0] = u[3];
             }
         }
-    if (FMT <= SMX_KV_INT8) {
-        const float *ks = c.ks + sbase + j0, *vs = c.vs + sbase + j0;
-#pragma unroll
-        for (int a = 0; a < 2 * NB; ++a) {
-            if (TAIL) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int tk = min(16 * a + 4 * g + r, last);
-                    x.ks[a].v[r] = ks[tk];
-                    x.vs[a].v[r] = vs[tk];
-                }
-            } else {
-                x.ks[a] = *reinterpret_cast<const CaF4*>(ks + 16 * a + 4 * g);
-                x.vs[a] = *reinterpret_cast<const CaF4*>(vs + 16 * a + 4 * g);
-            }
-        }
+}
+// the scale of key 16 a + 4 g + r of the block, from the lane of this row of 16 that holds it
+template <int K>
+__device__ __forceinline__ float ca_bcast(unsigned v) {
+    return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x150 + K, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float ca_scale(unsigned v, int a, int r) {         // (a, r: constants once unrolled)
+    switch (4 * a + r) {
+        case 0: return ca_bcast<0>(v);
+        case 1: return ca_bcast<1>(v);
+        case 2: return ca_bcast<2>(v);
+        case 3: return ca_bcast<3>(v);
+        case 4: return ca_bcast<4>(v);
+        case 5: return ca_bcast<5>(v);
+        case 6: return ca_bcast<6>(v);
+        case 7: return ca_bcast<7>(v);
+        case 8: return ca_bcast<8>(v);
+        case 9: return ca_bcast<9>(v);
+        case 10: return ca_bcast<10>(v);
+        case 11: return ca_bcast<11>(v);
+        case 12: return ca_bcast<12>(v);
+        case 13: return ca_bcast<13>(v);
+        case 14: return ca_bcast<14>(v);
+        default: return ca_bcast<15>(v);
     }
 }
 
 template <int FMT, int D, int MT, typename T>
-__global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p, CaPlan pl) {
-    enum { ES = CaFmt<FMT>::ES, NB = (ES * D == 64 && MT <= 2) ? 2 : 1, BK = 32 * NB, KF = D / 32, DT = D / 16,
+__global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void attn_cached_mfma(SmxCachedAttnParams p, CaPlan pl) {
+    enum { ES = CaFmt<FMT>::ES, NB = (ES * D == 64 && MT <= CA_NB2) ? 2 : 1,  BK = 32 * NB, KF = D / 32, DT = D / 16, 
            NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2 };
     typedef CaBlock<FMT, D, NB> Blk;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -147,9 +185,17 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
     const int nblk = (nmax + BK - 1) / BK, bps = (nblk + ns - 1) / ns;
     const int blk_end = min(nblk, (s + 1) * bps);
     const long long base = (long long)b * c.bs + (long long)hk * c.hs, sbase = (long long)b * c.sbs + (long long)hk * c.shs;
+    const CaView cv = {(const char*)c.k + base * ES, (const char*)c.v + base * ES, c.ks + sbase, c.vs + sbase, (int)c.ts * ES, nmax};
+    Blk x;
+    int blk = s * bps + w;
+    if (blk < blk_end) {
+        ca_load_k<FMT, D, NB>(x, cv, blk * BK);
+        ca_load_v<FMT, D, NB>(x, cv, blk * BK);
+    }
     // ---- this lane's rows
     int lim[MT], qpos[MT], hq[MT];
     unsigned qf[MT][NQ][KF][4];
+    const float scale2 = p.scale * CA_LOG2E;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int r = row0 + 16 * mt + i;
@@ -191,18 +237,9 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
     __shared__ float sm[CA_WAVES][16], sl[CA_WAVES][16];
     __shared__ __attribute__((aligned(16))) float so[CA_WAVES][16][D + 4];
 
-    Blk x, y;
-    int blk = s * bps + w;
-    if (blk < blk_end) {
-        if (blk * BK + BK <= nmax) ca_load<FMT, D, NB, false>(x, c, base, sbase, blk * BK, nmax);
-        else ca_load<FMT, D, NB, true>(x, c, base, sbase, blk * BK, nmax);
-    }
     for (; blk < blk_end; blk += CA_WAVES) {
-        const int j0 = blk * BK, jn = j0 + CA_WAVES * BK;
-        if (blk + CA_WAVES < blk_end) {
-            if (jn + BK <= nmax) ca_load<FMT, D, NB, false>(y, c, base, sbase, jn, nmax);
-            else ca_load<FMT, D, NB, true>(y, c, base, sbase, jn, nmax);
-        }
+        const int j0 = blk * BK;
+        const bool more = blk + CA_WAVES < blk_end;
         const bool masked = j0 + BK > nall;
         // ---- scores
         f32x4_t sc[MT][2 * NB];
@@ -211,7 +248,7 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
             unsigned kf[KF][4];
 #pragma unroll
             for (int q = 0; q < Blk::KC; ++q) {
-                const unsigned u[4] = {x.k[a][q].x, x.k[a][q].y, x.k[a][q].z, x.k[a][q].w};
+                const unsigned u[4] = {x.k[a][q][0], x.k[a][q][1], x.k[a][q][2], x.k[a][q][3]};
                 if (ES == 2) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) kf[q % KF][e] = u[e];
@@ -220,6 +257,9 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
                     for (int e = 0; e < 4; ++e) ca_cvt4<FMT>(u[e], kf[(2 * q + (e >> 1)) % KF][2 * (e & 1)], kf[(2 * q + (e >> 1)) % KF][2 * (e & 1) + 1]);
                 }
             }
+            float ksc[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ksc[r] = FMT <= SMX_KV_INT8 ? ca_scale(x.ks, a, r) * scale2 : scale2;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 sc[mt][a] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
@@ -228,12 +268,14 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
 #pragma unroll
                     for (int f = 0; f < KF; ++f) sc[mt][a] = ca_mfma(kf[f], qf[mt][n][f], sc[mt][a]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sc[mt][a][r] *= FMT <= SMX_KV_INT8 ? x.ks[a].v[r] * p.scale : p.scale;
+                for (int r = 0; r < 4; ++r) sc[mt][a][r] *= ksc[r];
                 if (p.rel_bias) {
                     const float* rb = p.rel_bias + (long long)hq[mt] * p.nrel;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        sc[mt][a][r] += rb[min(max(qpos[mt] - (pre ? 0 : np) - (j0 + 16 * a + 4 * g + r), 0), p.nrel - 1)];
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = fmaf(rb[min(max(qpos[mt] - (pre ? 0 : np) - (j0 + 16 * a + 4 * g + r), 0), p.nrel - 1)], CA_LOG2E, sc[mt][a][r]);
+                        sc[mt][a][r] = v < CA_LOWEST ? CA_LOWEST : v;          // (the lowest value times log2 e is no longer finite)
+                    }
                 }
                 if (masked)
 #pragma unroll
@@ -241,6 +283,7 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
                         if (j0 + 16 * a + 4 * g + r >= lim[mt]) sc[mt][a][r] = -INFINITY;
             }
         }
+        if (more) ca_load_k<FMT, D, NB>(x, cv, j0 + CA_WAVES * BK);
         // ---- reference
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -252,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
             if (__ballot(mx > m[mt] + CA_SLACK)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m[mt]);
-                const float al = mx == m[mt] ? 1.f : ca_exp(m[mt] - mx);        // (equal also while both are -inf)
+                const float al = mx == m[mt] ? 1.f : ca_exp2(m[mt] - mx);        // (equal also while both are -inf)
                 m[mt] = mx;
                 l[mt] *= al;
 #pragma unroll
@@ -262,15 +305,6 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
         // ---- probabilities and the second product, 32 keys at a time
         bool odd = false;                               // bf16: a value that is not finite among keys that some row must not see
         if (FMT == SMX_KV_BF16 && masked) {
-            if (j0 + BK > nmax) {
-#pragma unroll
-                for (int a = 0; a < 2 * NB; ++a)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (j0 + 16 * a + 4 * g + r >= nmax)
-#pragma unroll
-                            for (int q = 0; q < Blk::VW; ++q) x.v[a][r][q] = 0u;
-            }
             bool bad = false;
 #pragma unroll
             for (int a = 0; a < 2 * NB; ++a)
@@ -284,6 +318,11 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
 #pragma unroll
         for (int st = 0; st < NB; ++st) {
             unsigned pf[MT][NP][4];
+            float vsc[2][4];
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vsc[a][r] = FMT <= SMX_KV_INT8 ? ca_scale(x.vs, 2 * st + a, r) : 1.f;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
@@ -292,10 +331,10 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
                     float pr[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        pr[r] = ca_exp(sc[mt][2 * st + a][r] - ref);
+                        pr[r] = ca_exp2(sc[mt][2 * st + a][r] - ref);
                         l[mt] += pr[r];
                         if (FMT <= SMX_KV_INT8) {
-                            pr[r] *= x.vs[2 * st + a].v[r];
+                            pr[r] *= vsc[a][r];
                             if (masked && j0 + 32 * st + 16 * a + 4 * g + r >= lim[mt]) pr[r] = 0.f;
                         }
                     }
@@ -326,29 +365,30 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
                 }
             }
             if (FMT == SMX_KV_BF16 && odd) continue;
-            // V: registers of DPL elements per key -> per d-tile registers of two keys
-            unsigned vx[8][DT / 2];
+            // V, register by register of the keys: 4 (bf16: 2) d-tiles of two keys per register
+            enum { DR = 4 / ES };
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int q = 0; q < Blk::VW; ++q) {
+                unsigned vx[8][DR / 2];
 #pragma unroll
-                for (int q = 0; q < Blk::VW; ++q) {
+                for (int e = 0; e < 8; ++e) {
                     const unsigned u = x.v[2 * st + (e >> 2)][e & 3][q];
-                    if (ES == 2) vx[e][q % (DT / 2)] = u;
-                    else ca_cvt4<FMT>(u, vx[e][(2 * q) % (DT / 2)], vx[e][(2 * q + 1) % (DT / 2)]);
+                    if (ES == 2) vx[e][0] = u;
+                    else ca_cvt4<FMT>(u, vx[e][0], vx[e][DR / 2 - 1]);
                 }
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                unsigned vf[4];
+                for (int d = 0; d < DR; ++d) {
+                    unsigned vf[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    vf[q] = __builtin_amdgcn_perm(vx[2 * q + 1][d >> 1], vx[2 * q][d >> 1], (d & 1) ? 0x07060302u : 0x05040100u);
+                    for (int k = 0; k < 4; ++k) vf[k] = __builtin_amdgcn_perm(vx[2 * k + 1][d >> 1], vx[2 * k][d >> 1], (d & 1) ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int n = NP - 1; n >= 0; --n) acc[mt][d] = ca_mfma(vf, pf[mt][n], acc[mt][d]);
+                        for (int n = NP - 1; n >= 0; --n) acc[mt][DR * q + d] = ca_mfma(vf, pf[mt][n], acc[mt][DR * q + d]);
+                }
             }
         }
-        x = y;
+        if (more) ca_load_v<FMT, D, NB>(x, cv, j0 + CA_WAVES * BK);
     }
 
     // ---- the four waves meet: rows of 16, one tile at a time
@@ -376,7 +416,7 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
         for (int d = 0; d < DT; ++d) o[d] = 0.f;
 #pragma unroll
         for (int v = 0; v < CA_WAVES; ++v) {
-            const float mv = sm[v][row], f = mv == M ? 1.f : ca_exp(mv - M);
+            const float mv = sm[v][row], f = mv == M ? 1.f : ca_exp2(mv - M);
             L = fmaf(sl[v][row], f, L);
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] = fmaf(so[v][row][d0 + d], f, o[d]);
@@ -397,7 +437,7 @@ __global__ __launch_bounds__(256, 2) void attn_cached_mfma(SmxCachedAttnParams p
             T* out = reinterpret_cast<T*>(p.o) + bb * p.o_bs + t * p.o_ts + h * p.o_hs + d0;
 #pragma unroll
             for (int d = 0; d < DT; ++d) Cvt<T>::st(out + d, L == 0.f ? 0.f : o[d] * inv);
-            if (p.lse && d0 == 0) p.lse[((long long)bb * p.H + h) * p.Tq + t] = L == 0.f ? -INFINITY : M + logf(L);
+            if (p.lse && d0 == 0) p.lse[((long long)bb * p.H + h) * p.Tq + t] = ca_lse(M, L);
         }
     }
 }
@@ -409,39 +449,55 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
     const int lane = threadIdx.x & 63;
     if (id >= (long long)p.B * p.H * p.Tq) return;
     const int t = (int)(id % p.Tq), h = (int)(id / p.Tq % p.H), b = (int)(id / ((long long)p.Tq * p.H)), hk = h / pl.G;
-    float m = -INFINITY, l = 0.f, o[D / 64];
-#pragma unroll
-    for (int d = 0; d < D / 64; ++d) o[d] = 0.f;
+    // a lane holds four elements of every NG-th split: its loads depend on nothing but the weights
+    enum { LD = D / 4, NG = 64 / LD };
+    const int grp = lane / LD, dl = lane % LD * 4;
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int part = 0; part < 2; ++part) {
         const SmxKVCache& c = part ? p.own : p.pre;
         if (!c.k) continue;
         const int ns = part ? pl.nso : pl.nsp, e = part ? b : b / pl.R;
         const int r = (part ? 0 : b % pl.R * p.Tq * pl.G) + t * pl.G + h % pl.G;
         const long long it = (part ? pl.items_p : 0) + (((long long)(r / mt16) * c.B + e) * pl.Hkv + hk) * ns;
+        const float* po = pl.po + (it * mt16 + r % mt16) * D + dl;
+        const long long step = (long long)mt16 * D;
         // at most 64 splits: a lane holds one's maximum and sum
         float ms = -INFINITY, ls = 0.f;
         if (lane < ns) {
-            const float* q = pl.pml + 2 * ((it + lane) * mt16 + r % mt16);
-            ms = q[0];
-            ls = q[1];
+            const float2 q = *reinterpret_cast<const float2*>(pl.pml + 2 * ((it + lane) * mt16 + r % mt16));
+            ms = q.x;
+            ls = q.y;
         }
         const float M = fmaxf(m, wave_max(ms));
-        const float f0 = m == M ? 1.f : ca_exp(m - M), fs = ls == 0.f ? 0.f : ca_exp(ms - M);
+        const float f0 = m == M ? 1.f : ca_exp2(m - M), fs = ls == 0.f ? 0.f : ca_exp2(ms - M);
         l = l * f0 + wave_sum(ls * fs);
         m = M;
 #pragma unroll
-        for (int d = 0; d < D / 64; ++d) o[d] *= f0;
-        for (int s = 0; s < ns; ++s) {
-            const float f = __shfl(fs, s, 64);
-            if (f == 0.f) continue;                      // (nothing there, or too little to count)
-            const float* q = pl.po + ((it + s) * mt16 + r % mt16) * D;
+        for (int d = 0; d < 4; ++d) o[d] *= f0;
+        for (int s0 = 0; s0 < ns; s0 += 4 * NG) {
+            float4 q[4];
 #pragma unroll
-            for (int d = 0; d < D / 64; ++d) o[d] = fmaf(q[lane + 64 * d], f, o[d]);
+            for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const float4*>(po + min(s0 + NG * u + grp, ns - 1) * step);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int s = s0 + NG * u + grp;
+                const float v = __shfl(fs, s & 63, 64), f = s < ns ? v : 0.f;
+                o[0] = fmaf(q[u].x, f, o[0]);
+                o[1] = fmaf(q[u].y, f, o[1]);
+                o[2] = fmaf(q[u].z, f, o[2]);
+                o[3] = fmaf(q[u].w, f, o[3]);
+            }
         }
     }
-    T* out = reinterpret_cast<T*>(p.o) + b * p.o_bs + t * p.o_ts + h * p.o_hs;
-    const float inv = 1.f / l;
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) Cvt<T>::st(out + lane + 64 * d, l == 0.f ? 0.f : o[d] * inv);
-    if (p.lse && lane == 0) p.lse[id / p.Tq * p.Tq + t] = l == 0.f ? -INFINITY : m + logf(l);
+    for (int k = LD; k < 64; k <<= 1)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] += __shfl_xor(o[d], k, 64);
+    if (grp == 0) {
+        T* out = reinterpret_cast<T*>(p.o) + b * p.o_bs + t * p.o_ts + h * p.o_hs + dl;
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) Cvt<T>::st(out + d, l == 0.f ? 0.f : o[d] * inv);
+    }
+    if (p.lse && lane == 0) p.lse[id] = ca_lse(m, l);
 }

@@ -106,8 +106,14 @@ static bool ca_mfma_ok(const SmxCachedAttnParams& p) {
 }
 static int ca_cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 // splits of `cap` keys for `base` workgroups: enough of them to fill the chip, none with less than `least` keys
+#ifndef CA_WANT
+#define CA_WANT 512
+#endif
+#ifndef CA_LEAST
+#define CA_LEAST 512
+#endif
 static int ca_splits(long long base, int cap, int least) {
-    const long long want = ca_cdiv(1024, base), most = ca_cdiv(cap, least);
+    const long long want = ca_cdiv(CA_WANT, base), most = ca_cdiv(cap, least);
     const long long n = want < most ? want : most;
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
@@ -121,8 +127,8 @@ static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long lon
     pl.mbo = ca_cdiv(ro, 16 * mt);
     pl.mbp = ca_cdiv(rp, 16 * mt);
     const long long bo = (long long)pl.mbo * p.own.B * pl.Hkv, bp = (long long)pl.mbp * p.pre.B * pl.Hkv;
-    pl.nso = p.own.k ? ca_splits(bo, p.own.cap, 512) : 0;
-    pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, 512) : 0;
+    pl.nso = p.own.k ? ca_splits(bo, p.own.cap, CA_LEAST) : 0;
+    pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, CA_LEAST) : 0;
     pl.items_p = (int)(bp * pl.nsp);
     items = bp * pl.nsp + bo * pl.nso;
     pl.join = pl.nso + pl.nsp > 1;

@@ -1375,7 +1375,8 @@ def kv_read(cache, start, k, v):
 
 
 def _attention_cached_check(q, cache, klen, out, causal, scale, rel_bias, prefix, prefix_len):
-    """Every check of attention_cached that does not look at an address -> its parameter block, dtype and workspace size."""
+    """Every check of attention_cached that does not look at an address -> its parameter block, dtype, workspace size, and what the
+    outputs are allocated from."""
     name = "attention_cached"
     _on_device(name, q=q, out=out, rel_bias=rel_bias, klen=klen, prefix_len=prefix_len, cache=cache.k if cache is not None else None,
                prefix=prefix.k if prefix is not None else None)
@@ -1406,8 +1407,9 @@ def _attention_cached_check(q, cache, klen, out, causal, scale, rel_bias, prefix
     p.B, p.Tq, p.H, p.causal = B, Tq, H, int(bool(causal))
     p.scale = float(D ** -0.5 if scale is None else scale)
     dt = BF16 if q.dtype == torch.bfloat16 else F32
+    tail = (q.is_contiguous(), (B, H, Tq), q.device)
     if B == 0:
-        return bytes(p), dt, 0
+        return (bytes(p), dt, 0) + tail
     # (the library sizes the workspace from a whole block: the addresses only have to be there)
     p.own, p.pre = cache.desc if cache is not None else p.own, prefix.desc if prefix is not None else p.pre
     p.q = p.o = main.desc.k
@@ -1416,7 +1418,7 @@ def _attention_cached_check(q, cache, klen, out, causal, scale, rel_bias, prefix
     n = lib.smx_attention_cached_ws_bytes(C.byref(p), dt)
     L.check(0 if n >= 0 else n, "smx_attention_cached_ws_bytes")
     p.q = p.o = None
-    return bytes(p), dt, n
+    return (bytes(p), dt, n) + tail
 
 
 def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel_bias=None, prefix=None, prefix_len=None, want_lse=False):
@@ -1431,12 +1433,11 @@ def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel
     hit = _SIGNATURES.get(sig)
     if hit is None:
         hit = _remember(sig, _attention_cached_check(q, cache, klen, out, causal, scale, rel_bias, prefix, prefix_len))
-    tmpl, dt, n = hit
-    B, Tq, H, D = q.shape
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Tq), device=q.device) if want_lse else None
-    if B == 0:
+    tmpl, dt, n, dense, lse_shape, dev = hit
+    if out is None:          # (the allocations are a third of a short call's host time: empty_like is the quickest form)
+        out = torch.empty_like(q) if dense else torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(lse_shape, device=dev) if want_lse else None
+    if lse_shape[0] == 0:
         return out, lse
     p = L.CachedAttnParams.from_buffer_copy(tmpl)
     p.q, p.o = qp, op = q.data_ptr(), out.data_ptr()
@@ -1456,7 +1457,7 @@ def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel
         p.rel_bias = rel_bias.data_ptr()
     if n:
         # a workspace of its own per call, from the caching allocator: calls on other streams and captured graphs never share one
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
         p.ws, p.ws_bytes = ws.data_ptr(), n
     L.check(L.lib().smx_attention_cached(C.byref(p), dt, _stream()), "smx_attention_cached")
     return out, lse
@@ -1485,7 +1486,7 @@ def _verify_check(target, ids, draft, uniforms):
     p.ids_bs = ids.stride(0)
     p.B, p.n, p.V = B, n, V
     if B == 0:
-        return bytes(p), 0
+        return bytes(p), 0, B, n, target.device
     # (the workspace is sized from a whole block: the addresses only have to be there)
     p.target = p.accepted = p.token = target.data_ptr()
     p.u, p.ids = (p.target if uniforms is not None else None), (p.target if n else None)
@@ -1494,7 +1495,7 @@ def _verify_check(target, ids, draft, uniforms):
     nb = lib.smx_verify_draft_ws_bytes(C.byref(p))
     L.check(0 if nb >= 0 else nb, "smx_verify_draft_ws_bytes")
     p.target = p.accepted = p.token = p.u = p.ids = None
-    return bytes(p), nb
+    return bytes(p), nb, B, n, target.device
 
 
 def verify_draft(target, ids, draft=None, uniforms=None):
@@ -1508,22 +1509,21 @@ def verify_draft(target, ids, draft=None, uniforms=None):
     hit = _SIGNATURES.get(sig)
     if hit is None:
         hit = _remember(sig, _verify_check(target, ids, draft, uniforms))
-    tmpl, n = hit
-    B = target.shape[0]
-    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
-    token = torch.empty(B, dtype=torch.int64, device=target.device)
+    tmpl, nb, B, n, dev = hit
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    token = torch.empty(B, dtype=torch.int64, device=dev)
     if B == 0:
         return accepted, token
     p = L.VerifyParams.from_buffer_copy(tmpl)
     p.target, p.accepted, p.token = target.data_ptr(), accepted.data_ptr(), token.data_ptr()
-    if ids.shape[1]:
+    if n:
         p.ids = ids.data_ptr()
         if draft is not None:
             p.draft = draft.data_ptr()
     if uniforms is not None:
         p.u = uniforms.data_ptr()
-    if n:
-        ws = torch.empty(n, dtype=torch.uint8, device=target.device)
-        p.ws, p.ws_bytes = ws.data_ptr(), n
+    if nb:
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        p.ws, p.ws_bytes = ws.data_ptr(), nb
     L.check(L.lib().smx_verify_draft(C.byref(p), _stream()), "smx_verify_draft")
     return accepted, token

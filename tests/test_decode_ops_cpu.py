@@ -92,9 +92,11 @@ def test_attention_refuses_a_workspace_that_is_too_small(lib):
 
 
 @pytest.mark.parametrize("change", [dict(target=None), dict(accepted=None), dict(token=None), dict(B=0), dict(B=65536), dict(n=-1), dict(n=65), dict(V=0),
-                                    dict(ids=None), dict(u=None, draft=4096), dict(ws=None), dict(ws=4097), dict(ws_bytes=8)])
+                                    dict(ids=None), dict(u=None, draft=4096), dict(ws=None), dict(ws=4097), dict(ws_bytes=8),
+                                    dict(u=None, ws=None), dict(u=None, ws_bytes=8)])
 def test_verify_refused(lib, change):
-    p = L.VerifyParams(target=4096, u=4096, ids=4096, accepted=4096, token=4096, ws=4096, ws_bytes=1 << 20, B=2, n=3, V=50265)
+    # (two rows of 250 027: several workgroups a row, which need the workspace; so does the greedy form)
+    p = L.VerifyParams(target=4096, u=4096, ids=4096, accepted=4096, token=4096, ws=4096, ws_bytes=1 << 20, B=2, n=3, V=250027)
     for k, v in change.items():
         setattr(p, k, v)
     assert lib.smx_verify_draft(C.byref(p), None) == -22

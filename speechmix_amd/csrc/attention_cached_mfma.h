@@ -7,8 +7,8 @@
 // as the rounding of the output.
 //   K operand: a lane's 16 contiguous bytes of one key ARE eight k-indices of two (one for bf16) products; Q is loaded in the same order.
 //   V operand: a lane takes DPL = D / 16 neighbouring elements of each of its eight keys; one byte permute per register pairs two keys.
-// Softmax in units of log 2: every wave keeps its own reference m per row and moves it only when a score passes m + 16 (a wave-wide test):
-// probabilities stay below 2^16, and most blocks need no rescaling and no cross-lane maximum.  Four waves take every fourth block of BK keys, and meet in LDS;
+// Softmax in units of log 2: every wave keeps its own reference m per row and moves it only when a probability passes 2^16 (a wave-wide test): most
+// blocks need no rescaling and no cross-lane maximum.  Four waves take every fourth block of BK keys, and meet in LDS;
 // long caches are split over workgroups as well, whose unnormalised (m, l, O) a second kernel joins in a fixed order.
 #pragma once
 #include "kv_common.h"
@@ -17,16 +17,22 @@
 #ifndef CA_OCC
 #define CA_OCC 4
 #endif
+#ifndef CA_PF
+#define CA_PF 1
+#endif
 #ifndef CA_NB2
 #define CA_NB2 0
 #endif
 #define CA_LOG2E 1.44269504088896340736f
 #define CA_LN2 0.69314718055994530942f
-#define CA_SLACK 16.f             // a score may pass the reference by this much (log 2 units) before it moves
+#define CA_BIG 65536.f            // a score may pass the reference by this factor before it moves
 #define CA_LOWEST (-3.402823466e38f)
 
 // waves per SIMD the registers are held to
 constexpr int ca_occ(int es, int d, int mt, int qsize) { return qsize == 4 || (es == 2 && d == 128) || mt > 2 || (mt == 2 && d == 128) ? 2 : mt == 2 || d == 128 ? 3 : CA_OCC; }
+
+// blocks on the way at once
+constexpr int ca_depth(int es, int d, int mt, int qsize) { return CA_PF; }
 
 struct CaPlan {
     int G, Hkv, R;                // query heads per KV head; rows per prefix
@@ -63,6 +69,13 @@ __device__ __forceinline__ void ca_cvt4(unsigned u, unsigned& lo, unsigned& hi) 
     }
 }
 __device__ __forceinline__ float ca_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// bf16 pair product a . b + c
+__device__ __forceinline__ float ca_dot2(unsigned a, unsigned b, float c) {
+    union { unsigned u; smx_bf16x2_t v; } x, y;
+    x.u = a;
+    y.u = b;
+    return __builtin_amdgcn_fdot2_f32_bf16(x.v, y.v, c, false);
+}
 // log-sum-exp in natural units from a reference in log 2 units (a bias of the type's lowest value stays what it is)
 __device__ __forceinline__ float ca_lse(float m, float l) {
     return l == 0.f ? -INFINITY : m == CA_LOWEST ? CA_LOWEST : fmaf(m, CA_LN2, logf(l));
@@ -85,19 +98,20 @@ struct CaView {             // one head of a cache
     const float *ks, *vs;
     int tsb;                // bytes between tokens
     int nmax;
+    int koff, voff, soff;   // this lane's offsets within a block
 };
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t ca_rsrc(const void* base, long long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)(bytes < 0x7ffffff0ll ? bytes : 0x7ffffff0ll), 0x00020000);
 }
 template <int FMT, int D, int NB>
 __device__ __forceinline__ unsigned ca_load_scales(const float* s, const CaView& c, int j0) {
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    return __builtin_amdgcn_raw_buffer_load_b32(ca_rsrc(s + j0, (c.nmax - j0) * 4ll), 4 * (16 * (i >> 2) + 4 * g + (i & 3)), 0, 0);
+    return __builtin_amdgcn_raw_buffer_load_b32(ca_rsrc(s + j0, (c.nmax - j0) * 4ll), c.soff, 0, 0);
 }
 template <int FMT, int D, int NB>
 __device__ __forceinline__ void ca_load_k(CaBlock<FMT, D, NB>& x, const CaView& c, int j0) {
     typedef CaBlock<FMT, D, NB> B;
-    const int lane = threadIdx.x & 63, off = (lane & 15) * c.tsb + 16 * (lane >> 4);
+    int off = c.koff;
+    asm volatile("" : "+v"(off));       // (a sum per load: offsets kept from block to block would cost the registers of a tile)
     const __amdgpu_buffer_rsrc_t rs = ca_rsrc(c.k + (long long)j0 * c.tsb, (long long)(c.nmax - 1 - j0) * c.tsb + D * B::ES);
     if (FMT <= SMX_KV_INT8) x.ks = ca_load_scales<FMT, D, NB>(c.ks, c, j0);
 #pragma unroll
@@ -108,7 +122,8 @@ __device__ __forceinline__ void ca_load_k(CaBlock<FMT, D, NB>& x, const CaView& 
 template <int FMT, int D, int NB>
 __device__ __forceinline__ void ca_load_v(CaBlock<FMT, D, NB>& x, const CaView& c, int j0) {
     typedef CaBlock<FMT, D, NB> B;
-    const int lane = threadIdx.x & 63, off = 4 * (lane >> 4) * c.tsb + 4 * B::VW * (lane & 15);
+    int off = c.voff;
+    asm volatile("" : "+v"(off));
     const __amdgpu_buffer_rsrc_t rs = ca_rsrc(c.v + (long long)j0 * c.tsb, (long long)(c.nmax - 1 - j0) * c.tsb + D * B::ES);
     if (FMT <= SMX_KV_INT8) x.vs = ca_load_scales<FMT, D, NB>(c.vs, c, j0);
 #pragma unroll
@@ -158,7 +173,7 @@ __device__ __forceinline__ float ca_scale(unsigned v, int a, int r) {         //
 
 template <int FMT, int D, int MT, typename T>
 __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void attn_cached_mfma(SmxCachedAttnParams p, CaPlan pl) {
-    enum { ES = CaFmt<FMT>::ES, NB = (ES * D == 64 && MT <= CA_NB2) ? 2 : 1,  BK = 32 * NB, KF = D / 32, DT = D / 16, 
+    enum { ES = CaFmt<FMT>::ES, NB = (ES * D == 64 && MT <= CA_NB2) ? 2 : 1, PF = ca_depth(CaFmt<FMT>::ES, D, MT, sizeof(T)),  BK = 32 * NB, KF = D / 32, DT = D / 16, 
            NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2 };
     typedef CaBlock<FMT, D, NB> Blk;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -185,13 +200,16 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
     const int nblk = (nmax + BK - 1) / BK, bps = (nblk + ns - 1) / ns;
     const int blk_end = min(nblk, (s + 1) * bps);
     const long long base = (long long)b * c.bs + (long long)hk * c.hs, sbase = (long long)b * c.sbs + (long long)hk * c.shs;
-    const CaView cv = {(const char*)c.k + base * ES, (const char*)c.v + base * ES, c.ks + sbase, c.vs + sbase, (int)c.ts * ES, nmax};
-    Blk x;
+    const CaView cv = {(const char*)c.k + base * ES, (const char*)c.v + base * ES, c.ks + sbase, c.vs + sbase, (int)c.ts * ES, nmax,
+                       i * (int)c.ts * ES + 16 * g, 4 * g * (int)c.ts * ES + 4 * Blk::VW * i, 4 * (16 * (i >> 2) + 4 * g + (i & 3))};
+    Blk buf[PF];
     int blk = s * bps + w;
-    if (blk < blk_end) {
-        ca_load_k<FMT, D, NB>(x, cv, blk * BK);
-        ca_load_v<FMT, D, NB>(x, cv, blk * BK);
-    }
+#pragma unroll
+    for (int f = 0; f < PF; ++f)
+        if (blk + CA_WAVES * f < blk_end) {
+            ca_load_k<FMT, D, NB>(buf[f], cv, (blk + CA_WAVES * f) * BK);
+            ca_load_v<FMT, D, NB>(buf[f], cv, (blk + CA_WAVES * f) * BK);
+        }
     // ---- this lane's rows
     int lim[MT], qpos[MT], hq[MT];
     unsigned qf[MT][NQ][KF][4];
@@ -225,11 +243,13 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
             }
         }
     }
+    unsigned one_lo = 0x0000bf80u, one_hi = 0xbf800000u;          // (-1, 0), (0, -1)
+    asm("" : "+v"(one_lo), "+v"(one_hi));                       // (in registers: not every form of these constants means a pair)
     f32x4_t acc[MT][DT];
     float m[MT], l[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        m[mt] = -INFINITY;
+        m[mt] = CA_LOWEST;
         l[mt] = 0.f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[mt][d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
@@ -237,12 +257,13 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
     __shared__ float sm[CA_WAVES][16], sl[CA_WAVES][16];
     __shared__ __attribute__((aligned(16))) float so[CA_WAVES][16][D + 4];
 
-    for (; blk < blk_end; blk += CA_WAVES) {
+    auto block = [&](Blk& x) {
         const int j0 = blk * BK;
-        const bool more = blk + CA_WAVES < blk_end;
+        const bool more = blk + PF * CA_WAVES < blk_end;
         const bool masked = j0 + BK > nall;
         // ---- scores
-        f32x4_t sc[MT][2 * NB];
+        f32x4_t sc[MT][2 * NB];                         // q . codes; times ksc it is the score in log 2 units
+        float ksc[2 * NB][4];
 #pragma unroll
         for (int a = 0; a < 2 * NB; ++a) {
             unsigned kf[KF][4];
@@ -257,9 +278,8 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
                     for (int e = 0; e < 4; ++e) ca_cvt4<FMT>(u[e], kf[(2 * q + (e >> 1)) % KF][2 * (e & 1)], kf[(2 * q + (e >> 1)) % KF][2 * (e & 1) + 1]);
                 }
             }
-            float ksc[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) ksc[r] = FMT <= SMX_KV_INT8 ? ca_scale(x.ks, a, r) * scale2 : scale2;
+            for (int r = 0; r < 4; ++r) ksc[a][r] = FMT <= SMX_KV_INT8 ? ca_scale(x.ks, a, r) * scale2 : scale2;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 sc[mt][a] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
@@ -267,43 +287,28 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
                 for (int n = NQ - 1; n >= 0; --n)       // small parts first
 #pragma unroll
                     for (int f = 0; f < KF; ++f) sc[mt][a] = ca_mfma(kf[f], qf[mt][n][f], sc[mt][a]);
+                if (masked || p.rel_bias) {             // (uniform; sc is the score itself from here on: its factor becomes 1 below)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sc[mt][a][r] *= ksc[r];
-                if (p.rel_bias) {
-                    const float* rb = p.rel_bias + (long long)hq[mt] * p.nrel;
+                    for (int r = 0; r < 4; ++r) sc[mt][a][r] *= ksc[a][r];
+                    if (p.rel_bias) {
+                        const float* rb = p.rel_bias + (long long)hq[mt] * p.nrel;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float v = fmaf(rb[min(max(qpos[mt] - (pre ? 0 : np) - (j0 + 16 * a + 4 * g + r), 0), p.nrel - 1)], CA_LOG2E, sc[mt][a][r]);
-                        sc[mt][a][r] = v < CA_LOWEST ? CA_LOWEST : v;          // (the lowest value times log2 e is no longer finite)
+                        for (int r = 0; r < 4; ++r) {
+                            const float v = fmaf(rb[min(max(qpos[mt] - (pre ? 0 : np) - (j0 + 16 * a + 4 * g + r), 0), p.nrel - 1)], CA_LOG2E, sc[mt][a][r]);
+                            sc[mt][a][r] = v < CA_LOWEST ? CA_LOWEST : v;          // (the lowest value times log2 e is no longer finite)
+                        }
                     }
-                }
-                if (masked)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (j0 + 16 * a + 4 * g + r >= lim[mt]) sc[mt][a][r] = -INFINITY;
+                }
             }
+            if (masked || p.rel_bias)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) ksc[a][r] = 1.f;
         }
-        if (more) ca_load_k<FMT, D, NB>(x, cv, j0 + CA_WAVES * BK);
-        // ---- reference
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            float mx = sc[mt][0][0];
-#pragma unroll
-            for (int a = 0; a < 2 * NB; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[mt][a][r]);
-            if (__ballot(mx > m[mt] + CA_SLACK)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m[mt]);
-                const float al = mx == m[mt] ? 1.f : ca_exp2(m[mt] - mx);        // (equal also while both are -inf)
-                m[mt] = mx;
-                l[mt] *= al;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) acc[mt][d] *= al;
-            }
-        }
-        // ---- probabilities and the second product, 32 keys at a time
-        bool odd = false;                               // bf16: a value that is not finite among keys that some row must not see
+        if (more) ca_load_k<FMT, D, NB>(x, cv, j0 + PF * CA_WAVES * BK);
+        bool odd = false;                               // bf16: a value that is not finite in a block of which some row must not see all
         if (FMT == SMX_KV_BF16 && masked) {
             bool bad = false;
 #pragma unroll
@@ -313,58 +318,80 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
 #pragma unroll
                     for (int q = 0; q < Blk::VW; ++q)
                         bad |= (x.v[a][r][q] & 0x7f80u) == 0x7f80u || (x.v[a][r][q] & 0x7f800000u) == 0x7f800000u;
-            odd = __ballot(bad) != 0;
+            odd = causal && __ballot(bad) != 0;
+            if (odd)                                    // (the product leaves them out; the rows that do see them get them below)
+#pragma unroll
+                for (int a = 0; a < 2 * NB; ++a)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int q = 0; q < Blk::VW; ++q) {
+                            if ((x.v[a][r][q] & 0x7f80u) == 0x7f80u) x.v[a][r][q] &= 0xffff0000u;
+                            if ((x.v[a][r][q] & 0x7f800000u) == 0x7f800000u) x.v[a][r][q] &= 0xffffu;
+                        }
         }
+        float vsc[2 * NB][4];
 #pragma unroll
-        for (int st = 0; st < NB; ++st) {
-            unsigned pf[MT][NP][4];
-            float vsc[2][4];
+        for (int a = 0; a < 2 * NB; ++a)
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+            for (int r = 0; r < 4; ++r) vsc[a][r] = FMT <= SMX_KV_INT8 ? ca_scale(x.vs, a, r) : 1.f;
+        // ---- probabilities: one fused product and difference, one exponential.  A probability above 2^16 (also the first ever: the reference
+        // starts at the lowest value) sends the row's wave back to the scores for a new reference.
+        unsigned pf[MT][NB][NP][4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) vsc[a][r] = FMT <= SMX_KV_INT8 ? ca_scale(x.vs, 2 * st + a, r) : 1.f;
+        for (int mt = 0; mt < MT; ++mt) {
+            f32x4_t pr[2 * NB];
+            float big = 0.f;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
+            for (int a = 0; a < 2 * NB; ++a)
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    float pr[4];
+                for (int r = 0; r < 4; ++r) {
+                    pr[a][r] = ca_exp2(fmaf(sc[mt][a][r], ksc[a][r], -m[mt]));
+                    big = fmaxf(big, pr[a][r]);
+                }
+            if (__ballot(big > CA_BIG)) {
+                float mx = m[mt];
+#pragma unroll
+                for (int a = 0; a < 2 * NB; ++a)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[mt][a][r] * ksc[a][r]);
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float al = mx == m[mt] ? 1.f : ca_exp2(m[mt] - mx);
+                m[mt] = mx;
+                l[mt] *= al;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[mt][d] *= al;
+#pragma unroll
+                for (int a = 0; a < 2 * NB; ++a)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) pr[a][r] = ca_exp2(fmaf(sc[mt][a][r], ksc[a][r], -mx));
+            }
+#pragma unroll
+            for (int a = 0; a < 2 * NB; ++a) {
+                l[mt] += (pr[a][0] + pr[a][1]) + (pr[a][2] + pr[a][3]);
+                if (FMT <= SMX_KV_INT8)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        pr[r] = ca_exp2(sc[mt][2 * st + a][r] - ref);
-                        l[mt] += pr[r];
-                        if (FMT <= SMX_KV_INT8) {
-                            pr[r] *= vsc[a][r];
-                            if (masked && j0 + 32 * st + 16 * a + 4 * g + r >= lim[mt]) pr[r] = 0.f;
-                        }
-                    }
-                    if (FMT == SMX_KV_BF16 && odd) {
-                        // rare: key by key, so that a zero probability never meets an infinity
-                        for (int k = 0; k < 16; ++k) {
-                            const int src = (k >> 2) * 16 + i, j = j0 + 32 * st + 16 * a + k;
-                            const float p0 = __shfl(pr[0], src, 64), p1 = __shfl(pr[1], src, 64), p2 = __shfl(pr[2], src, 64), p3 = __shfl(pr[3], src, 64);
-                            const float pk = (k & 2) ? ((k & 1) ? p3 : p2) : ((k & 1) ? p1 : p0);
-                            if (j < lim[mt]) {
-                                const bf16_t* v = reinterpret_cast<const bf16_t*>(c.v) + base + (long long)j * c.ts;
-#pragma unroll
-                                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                                    for (int r = 0; r < 4; ++r) acc[mt][d][r] = fmaf(pk, bf2f(v[DT * (4 * g + r) + d]), acc[mt][d][r]);
-                            }
-                        }
+                        pr[a][r] *= vsc[a][r];
+                        if (masked && j0 + 16 * a + 4 * g + r >= lim[mt]) pr[a][r] = 0.f;                  // (its scale may be anything)
                     }
 #pragma unroll
-                    for (int n = 0; n < NP; ++n)
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const unsigned h = pack_bf2(pr[2 * e], pr[2 * e + 1]);
-                            pf[mt][n][2 * a + e] = h;
-                            pr[2 * e] -= __uint_as_float(h << 16);
-                            pr[2 * e + 1] -= __uint_as_float(h & 0xffff0000u);
+                    for (int n = 0; n < NP; ++n) {
+                        const unsigned h = pack_bf2(pr[a][2 * e], pr[a][2 * e + 1]);
+                        pf[mt][a >> 1][n][2 * (a & 1) + e] = h;
+                        if (n + 1 < NP) {               // what h leaves over: -1 * its half + the number, one instruction
+                            pr[a][2 * e] = ca_dot2(h, one_lo, pr[a][2 * e]);
+                            pr[a][2 * e + 1] = ca_dot2(h, one_hi, pr[a][2 * e + 1]);
                         }
-                }
+                    }
             }
-            if (FMT == SMX_KV_BF16 && odd) continue;
+        }
+        // ---- the second product, 32 keys at a time
+#pragma unroll
+        for (int st = 0; st < NB; ++st) {
             // V, register by register of the keys: 4 (bf16: 2) d-tiles of two keys per register
             enum { DR = 4 / ES };
 #pragma unroll
@@ -384,11 +411,37 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int n = NP - 1; n >= 0; --n) acc[mt][DR * q + d] = ca_mfma(vf, pf[mt][n], acc[mt][DR * q + d]);
+                        for (int n = NP - 1; n >= 0; --n) acc[mt][DR * q + d] = ca_mfma(vf, pf[mt][st][n], acc[mt][DR * q + d]);
                 }
             }
         }
-        if (more) ca_load_v<FMT, D, NB>(x, cv, j0 + CA_WAVES * BK);
+        if (FMT == SMX_KV_BF16 && odd) {
+            for (int k = 0; k < BK; ++k) {              // rare: key by key, the elements that are not finite, for the rows that see the key
+                const int j = j0 + k, src = ((k >> 2) & 3) * 16 + i, wd = 2 * ((k >> 4) & 1) + ((k >> 1) & 1);
+                const bf16_t* v = reinterpret_cast<const bf16_t*>(c.v) + base + (long long)min(j, nmax - 1) * c.ts;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const unsigned w0 = pf[mt][0][0][0], w1 = pf[mt][0][0][1], w2 = pf[mt][0][0][2], w3 = pf[mt][0][0][3];
+                    const unsigned u01 = wd & 1 ? w1 : w0, u23 = wd & 1 ? w3 : w2, u = (unsigned)__shfl((int)(wd & 2 ? u23 : u01), src, 64);
+                    const float pk = __uint_as_float(k & 1 ? u & 0xffff0000u : u << 16);
+                    if (j < lim[mt])
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float f = bf2f(v[DT * (4 * g + r) + d]);
+                                if (!(fabsf(f) < INFINITY)) acc[mt][d][r] = fmaf(pk, f, acc[mt][d][r]);
+                            }
+                }
+            }
+        }
+        if (more) ca_load_v<FMT, D, NB>(x, cv, j0 + PF * CA_WAVES * BK);
+        blk += CA_WAVES;
+    };
+    while (blk < blk_end) {
+#pragma unroll
+        for (int f = 0; f < PF; ++f)
+            if (f == 0 || blk < blk_end) block(buf[f]);
     }
 
     // ---- the four waves meet: rows of 16, one tile at a time
@@ -409,7 +462,7 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
                     make_float4(acc[mt][d][r], acc[mt][d + 1][r], acc[mt][d + 2][r], acc[mt][d + 3][r]);
         __syncthreads();
         const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * DT, r = row0 + 16 * mt + row;
-        float M = -INFINITY, L = 0.f, o[DT];
+        float M = CA_LOWEST, L = 0.f, o[DT];
 #pragma unroll
         for (int v = 0; v < CA_WAVES; ++v) M = fmaxf(M, sm[v][row]);
 #pragma unroll

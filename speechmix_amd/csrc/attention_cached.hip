@@ -105,17 +105,13 @@ static bool ca_mfma_ok(const SmxCachedAttnParams& p) {
     return true;
 }
 static int ca_cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
-// splits of `cap` keys for `base` workgroups: enough of them to fill the chip, none with less than `least` keys
-#ifndef CA_WANT
-#define CA_WANT 512
-#endif
-#ifndef CA_LEAST
-#define CA_LEAST 512
-#endif
-static int ca_splits(long long base, int cap, int least) {
-    const long long want = ca_cdiv(CA_WANT, base), most = ca_cdiv(cap, least);
-    const long long n = want < most ? want : most;
-    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+// Splits of `cap` keys for `base` workgroups: up to `want` workgroups.  A split costs the second launch (5 us) and its partial rows, so it has to take
+// at least 512 keys, and 2 048 where the rows alone already give the chip a workgroup per CU (32 x 16 heads x 777 keys: one launch 13 us,
+// two splits 14 + 4; 16 x 16 heads x 8 192 int8 keys: 84 us unsplit, 52 in four).
+static int ca_splits(long long base, int cap, long long want) {
+    const long long n = want / base, most = ca_cdiv(cap, base >= 256 ? 2048 : 512);
+    const long long m = n < most ? n : most;
+    return (int)(m < 1 ? 1 : m > 64 ? 64 : m);
 }
 static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long long& items) {
     const SmxKVCache& m = p.own.k ? p.own : p.pre;
@@ -127,8 +123,11 @@ static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long lon
     pl.mbo = ca_cdiv(ro, 16 * mt);
     pl.mbp = ca_cdiv(rp, 16 * mt);
     const long long bo = (long long)pl.mbo * p.own.B * pl.Hkv, bp = (long long)pl.mbp * p.pre.B * pl.Hkv;
-    pl.nso = p.own.k ? ca_splits(bo, p.own.cap, CA_LEAST) : 0;
-    pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, CA_LEAST) : 0;
+    // what is resident at once: four workgroups per CU of the small form, two or three of the others; a prefix gets what its rows' own keys leave
+    const long long want = mt == 1 && m.D == 64 ? 1024 : 512;
+    pl.nso = p.own.k ? ca_splits(bo, p.own.cap, want) : 0;
+    const long long left = want - bo * pl.nso;
+    pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, left > want / 2 ? left : want / 2) : 0;
     pl.items_p = (int)(bp * pl.nsp);
     items = bp * pl.nsp + bo * pl.nso;
     pl.join = pl.nso + pl.nsp > 1;

@@ -171,23 +171,23 @@ __device__ __forceinline__ float ca_scale(unsigned v, int a, int r) {         //
     }
 }
 
-template <int FMT, int D, int MT, typename T>
-__global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void attn_cached_mfma(SmxCachedAttnParams p, CaPlan pl) {
-    enum { ES = CaFmt<FMT>::ES, NB = (ES * D == 64 && MT <= CA_NB2) ? 2 : 1, PF = ca_depth(CaFmt<FMT>::ES, D, MT, sizeof(T)),  BK = 32 * NB, KF = D / 32, DT = D / 16, 
+template <int D> struct CaShared {       // where the four waves meet
+    float m[CA_WAVES][16], l[CA_WAVES][16];
+    __attribute__((aligned(16))) float o[CA_WAVES][16][D + 4];
+};
+struct CaItem { bool pre; int s, hk, b, row0; };      // key split, KV head, batch entry, first row
+
+// One work item: 16 * MT rows (as many as there are of the kernel's 16 * MTB) over one split of the keys
+template <int FMT, int D, int MT, int MTB, typename T>
+__device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPlan& pl, const CaItem& it, CaShared<D>& sh) {
+    enum { ES = CaFmt<FMT>::ES, NB = (ES * D == 64 && MT <= CA_NB2) ? 2 : 1, PF = ca_depth(CaFmt<FMT>::ES, D, MT, sizeof(T)), BK = 32 * NB, KF = D / 32, DT = D / 16,
            NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2 };
     typedef CaBlock<FMT, D, NB> Blk;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    // ---- which rows, which keys
-    int id = blockIdx.x;
-    const bool pre = id < pl.items_p;
-    if (!pre) id -= pl.items_p;
+    const bool pre = it.pre;
+    const int s = it.s, hk = it.hk, b = it.b, row0 = it.row0;
     const SmxKVCache& c = pre ? p.pre : p.own;
     const int ns = pre ? pl.nsp : pl.nso;
-    const int s = id % ns;
-    id /= ns;
-    const int hk = id % pl.Hkv;
-    id /= pl.Hkv;
-    const int b = id % c.B, row0 = id / c.B * (16 * MT);
     const int per = p.Tq * pl.G, nrows = (pre ? pl.R : 1) * per, b0 = pre ? b * pl.R : b;
     int np = 0, nk = 0;
     if (p.pre.k) np = p.plen ? min(max(p.plen[b0 / pl.R], 0), p.pre.cap) : p.pre.cap;
@@ -254,9 +254,6 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[mt][d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-    __shared__ float sm[CA_WAVES][16], sl[CA_WAVES][16];
-    __shared__ __attribute__((aligned(16))) float so[CA_WAVES][16][D + 4];
-
     auto block = [&](Blk& x) {
         const int j0 = blk * BK;
         const bool more = blk + PF * CA_WAVES < blk_end;
@@ -451,31 +448,31 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
         l[mt] += __shfl_xor(l[mt], 32, 64);
         if (mt) __syncthreads();
         if (g == 0) {
-            sm[w][i] = m[mt];
-            sl[w][i] = l[mt];
+            sh.m[w][i] = m[mt];
+            sh.l[w][i] = l[mt];
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int d = 0; d < DT; d += 4)
-                *reinterpret_cast<float4*>(&so[w][i][DT * (4 * g + r) + d]) =
+                *reinterpret_cast<float4*>(&sh.o[w][i][DT * (4 * g + r) + d]) =
                     make_float4(acc[mt][d][r], acc[mt][d + 1][r], acc[mt][d + 2][r], acc[mt][d + 3][r]);
         __syncthreads();
         const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * DT, r = row0 + 16 * mt + row;
         float M = CA_LOWEST, L = 0.f, o[DT];
 #pragma unroll
-        for (int v = 0; v < CA_WAVES; ++v) M = fmaxf(M, sm[v][row]);
+        for (int v = 0; v < CA_WAVES; ++v) M = fmaxf(M, sh.m[v][row]);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = 0.f;
 #pragma unroll
         for (int v = 0; v < CA_WAVES; ++v) {
-            const float mv = sm[v][row], f = mv == M ? 1.f : ca_exp2(mv - M);
-            L = fmaf(sl[v][row], f, L);
+            const float mv = sh.m[v][row], f = mv == M ? 1.f : ca_exp2(mv - M);
+            L = fmaf(sh.l[v][row], f, L);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] = fmaf(so[v][row][d0 + d], f, o[d]);
+            for (int d = 0; d < DT; ++d) o[d] = fmaf(sh.o[v][row][d0 + d], f, o[d]);
         }
         if (pl.join) {
-            const long long pr = (long long)blockIdx.x * (16 * MT) + 16 * mt + row;
+            const long long pr = (long long)blockIdx.x * (16 * MTB) + 16 * mt + row;
             if (r < nrows) {
                 if (d0 == 0) {
                     pl.pml[2 * pr] = M;
@@ -493,6 +490,25 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
             if (p.lse && d0 == 0) p.lse[((long long)bb * p.H + h) * p.Tq + t] = ca_lse(M, L);
         }
     }
+}
+
+template <int FMT, int D, int MT, typename T>
+__global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void attn_cached_mfma(SmxCachedAttnParams p, CaPlan pl) {
+    __shared__ CaShared<D> sh;
+    int id = blockIdx.x;
+    CaItem it;
+    it.pre = id < pl.items_p;
+    if (!it.pre) id -= pl.items_p;
+    const int ns = it.pre ? pl.nsp : pl.nso, cb = it.pre ? p.pre.B : p.own.B, per = p.Tq * pl.G, nrows = it.pre ? pl.R * per : per;
+    it.s = id % ns;
+    id /= ns;
+    it.hk = id % pl.Hkv;
+    id /= pl.Hkv;
+    it.b = id % cb;
+    it.row0 = id / cb * (16 * MT);
+    // (a batch behind a prefix: the prefix's many rows choose MT, a row's own keys have few)
+    if (MT > 1 && nrows - it.row0 <= 16) ca_body<FMT, D, 1, MT, T>(p, pl, it, sh);
+    else ca_body<FMT, D, MT, MT, T>(p, pl, it, sh);
 }
 
 // O = sum over the splits of both parts, in order.  One wave per (row, head, query).

@@ -1404,8 +1404,8 @@ def _attention_cached_check(q, cache, klen, out, causal, scale, rel_bias, prefix
         _need(rel_bias.dtype == torch.float32 and rel_bias.dim() == 2 and rel_bias.shape[0] == H and rel_bias.shape[1] > 0 and rel_bias.is_contiguous(),
               f"{name}: rel_bias must be contiguous fp32 [H, n]")
         p.nrel = rel_bias.shape[1]
-    p.B, p.Tq, p.H, p.causal = B, Tq, H, int(bool(causal))
-    p.scale = float(D ** -0.5 if scale is None else scale)
+    p.B, p.Tq, p.H, p.causal = B, Tq, H, int(causal)
+    p.scale = D ** -0.5 if scale is None else scale
     dt = BF16 if q.dtype == torch.bfloat16 else F32
     tail = (q.is_contiguous(), (B, H, Tq), q.device)
     if B == 0:
@@ -1428,6 +1428,7 @@ def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel
     tokens among themselves.  H may be a multiple of the caches' heads.  scale: D ** -0.5 unless given.  rel_bias fp32 [H, n]: bias by the
     distance query - key, clamped to 0 .. n - 1.  A query that sees no key gives zeros and lse = -inf.
     -> (out [B, Tq, H, D] of q's type, lse fp32 [B, H, Tq] or None)."""
+    causal, scale = bool(causal), None if scale is None else float(scale)          # (values, not objects, in the signature)
     sig = (_sig(q), cache.signature if cache is not None else None, prefix.signature if prefix is not None else None, torch._C._cuda_getDevice(),
            _sig(klen), _sig(prefix_len), _sig(out), _sig(rel_bias), causal, scale)
     hit = _SIGNATURES.get(sig)

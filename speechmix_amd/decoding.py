@@ -5,7 +5,10 @@ sampled rows per clip, a drafting model - need what that loop cannot do: rows at
 step, and cross-attention keys that the rows of a clip share (HF's `generate(num_return_sequences=, do_sample=, temperature=,
 assistant_model=)`; the reference's loops are greedy, ref:train.py:18-34, and its HF twin hands generation to HF, ref:speechmix/hf_model.py:354-375).
 """
+import gc
 import math
+import os
+import warnings
 
 import torch
 
@@ -55,6 +58,8 @@ class CachedDecoder:
         self.head_alpha = (self.d ** -0.5 if (self.t5 and lc.tie_word_embeddings) else 1.0) * logit_scale
         self.flb = st.module.get_buffer(lp + "final_logits_bias").view(-1) * logit_scale if not self.t5 else None
         self.lens = torch.zeros(self.N, dtype=torch.int32, device=eng.dev)
+        self.use_graphs = eng.dev.type == "cuda" and eng.dt == BF16 and os.environ.get("SMX_DECODE_GRAPH", "1") != "0"
+        self.graphs, self.warm = {}, set()
         self.rel = None
         if self.t5:            # row `capacity - 1` of the bias sees every distance: [H, capacity], indexed by query - key
             self.rel = eng._t5_bias("decoder", capacity, capacity)[0][:, capacity - 1].flip(-1).contiguous()
@@ -80,8 +85,40 @@ class CachedDecoder:
         return sum(c.bytes() for c in self.own + self.cross)
 
     def step(self, ids):
-        """ids int64 [N, Tq] -> logits fp32 [N, Tq, V] (a view of rows of Vp).  Rows past the capacity (finished ones that are still fed) write
-        nothing and give logits without meaning."""
+        """ids int64 [N, Tq] -> logits fp32 [N, Tq, V] (a view of rows of Vp, valid until the next step of as many tokens).  Rows past the
+        capacity (finished ones that are still fed) write nothing and give logits without meaning.
+
+        Nothing in a step but `lens` and the ids depends on the position, and both are in device memory: the second step of a width is
+        captured into a HIP graph (its kernel picks are made by then) and replayed from then on, as greedy_decode does per position
+        (bf16; SMX_DECODE_GRAPH=0: off)."""
+        Tq = ids.shape[1]
+        g = self.graphs.get(Tq)
+        if g is None and Tq in self.warm and self.use_graphs:
+            g = self.graphs[Tq] = self._capture(ids)
+        if not g:                                       # (False: capture was refused, this width stays eager)
+            self.warm.add(Tq)
+            return self._step(ids)
+        graph, buf, logits = g
+        buf.copy_(ids)
+        graph.replay()
+        return logits
+
+    def _capture(self, ids):
+        graph, buf = torch.cuda.CUDAGraph(), ids.clone()
+        gc_was = gc.isenabled()
+        gc.disable()                                    # (no finaliser may run on a capturing thread: graphs.StepGraphs.capture)
+        try:
+            with torch.cuda.graph(graph, capture_error_mode=os.environ.get("SMX_CAPTURE_MODE", "thread_local")):
+                logits = self._step(buf)
+        except RuntimeError as e:
+            warnings.warn(f"CachedDecoder: HIP graph capture failed ({e}); decoding eagerly")
+            return False
+        finally:
+            if gc_was:
+                gc.enable()
+        return graph, buf, logits
+
+    def _step(self, ids):
         eng, lc = self.eng, self.eng.lc
         N, Tq = ids.shape
         M, d, H, hd, eps, t5 = N * Tq, self.d, self.H, self.hd, self.eps, self.t5
@@ -156,23 +193,24 @@ def decode(dec, max_new_tokens, start_id, eos_id, pad_id, sample=False, generato
     def uniforms(k):
         return torch.rand(N, k, device=dev, generator=generator) if sample else None
     none = torch.empty(N, 0, dtype=torch.int64, device=dev)
+    q = torch.empty(N, n, dec.V, device=dev) if sample and n else None
     steps = 0
     while True:
-        ids, q = [tok], []
-        for _ in range(n):
+        ids = [tok]
+        for i in range(n):
             lg = draft.step(ids[-1])
             pr = draft.probabilities(lg) if sample else lg
             nxt = ops.verify_draft(pr, none, None, uniforms(1))[1]            # (nothing drafted: a plain draw / arg max)
             draft.lens += 1
             ids.append(nxt[:, None])
             if sample:
-                q.append(pr)
+                q[:, i] = pr[:, 0]
         if n:                                                                 # the last draft's keys, in case it is accepted
             draft.step(ids[-1])
         fed = torch.cat(ids, 1)
         lg = dec.step(fed)
         pr = dec.probabilities(lg) if sample else lg
-        acc, nxt = ops.verify_draft(pr, fed[:, 1:], torch.cat(q, 1) if q else None, uniforms(n + 1))
+        acc, nxt = ops.verify_draft(pr, fed[:, 1:], q, uniforms(n + 1))
         steps += 1
         # accepted drafts, then the next token; what stands behind it is overwritten by the next step
         acc = acc.long()

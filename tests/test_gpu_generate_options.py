@@ -159,6 +159,37 @@ def test_a_drafting_model_changes_the_steps_not_the_tokens(lm, dtype):
                 assert model.last_decode_steps == math.ceil(14 / 5)
 
 
+@pytest.mark.parametrize("lm", [BART, T5], ids=["bart", "t5"])
+def test_replayed_steps_equal_eager_ones(lm, monkeypatch):
+    """bf16 steps are captured at their second use and replayed: the same bits as eager steps, over several replays with other work between them,
+    for one and for several tokens, on rows at different lengths; and generate emits the same tokens either way."""
+    from speechmix_amd.decoding import CachedDecoder
+    model = _model(lm, "bf16")
+    with torch.no_grad():
+        enc, B, S = model._speech_encode(_wave(2))
+        fed = torch.randint(4, 200, (4, 3), generator=torch.Generator().manual_seed(5)).to(model.device)
+        outs = []
+        for flag in ("0", "1"):
+            monkeypatch.setenv("SMX_DECODE_GRAPH", flag)
+            dec = CachedDecoder(model.engine, enc, B, S, 2, 40, "fp8")
+            got = []
+            for k in range(6):
+                for ids in (fed[:, :1].contiguous(), (fed + k) % 200):
+                    got.append(dec.step(ids).clone())
+                    dec.lens += torch.tensor([1, 2, 1, ids.shape[1]], dtype=torch.int32, device=model.device).clamp_max(ids.shape[1])
+                    torch.randn(1000, device=model.device).sum().item()
+            assert bool(dec.graphs) == (flag == "1") and all(dec.graphs.values())
+            outs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    model.decoder_model.config.eos_token_id = -1
+    kw = dict(max_length=11, kv_cache="int8", do_sample=True, num_return_sequences=3, assistant_model=model, num_assistant_tokens=2)
+    rows = []
+    for flag in ("0", "1"):
+        monkeypatch.setenv("SMX_DECODE_GRAPH", flag)
+        rows.append(model.generate(_wave(2), generator=torch.Generator(device=model.device).manual_seed(4), **kw))
+    assert rows[0] == rows[1]
+
+
 @pytest.mark.parametrize("kv", [None, "fp8"])
 def test_sampled_rows(kv):
     """Rows per clip, seeds, temperatures."""

@@ -76,6 +76,11 @@ __device__ __forceinline__ float ca_dot2(unsigned a, unsigned b, float c) {
     y.u = b;
     return __builtin_amdgcn_fdot2_f32_bf16(x.v, y.v, c, false);
 }
+// a bias in log 2 units (the type's lowest value times log2 e is no longer finite; -inf and NaN stay)
+__device__ __forceinline__ float ca_bias2(float b) {
+    const float v = b * CA_LOG2E;
+    return v < CA_LOWEST && b >= CA_LOWEST ? CA_LOWEST : v;
+}
 // log-sum-exp in natural units from a reference in log 2 units (a bias of the type's lowest value stays what it is)
 __device__ __forceinline__ float ca_lse(float m, float l) {
     return l == 0.f ? -INFINITY : m == CA_LOWEST ? CA_LOWEST : fmaf(m, CA_LN2, logf(l));
@@ -211,6 +216,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             ca_load_v<FMT, D, NB>(buf[f], cv, (blk + CA_WAVES * f) * BK);
         }
     // ---- this lane's rows
+    const int kpos0 = pre ? 0 : np;                     // position of key 0
     int lim[MT], qpos[MT], hq[MT];
     unsigned qf[MT][NQ][KF][4];
     const float scale2 = p.scale * CA_LOG2E;
@@ -285,19 +291,28 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
                     for (int f = 0; f < KF; ++f) sc[mt][a] = ca_mfma(kf[f], qf[mt][n][f], sc[mt][a]);
                 if (masked || p.rel_bias) {             // (uniform; sc is the score itself from here on: its factor becomes 1 below)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) sc[mt][a][r] *= ksc[a][r];
                     if (p.rel_bias) {
                         const float* rb = p.rel_bias + (long long)hq[mt] * p.nrel;
+                        // keys so far back that every distance of the tile is beyond the table: its last value, without the gathers
+                        if (__ballot(qpos[mt] - kpos0 - (j0 + 16 * a + 15) < p.nrel - 1) == 0) {
+                            const float end = ca_bias2(rb[p.nrel - 1]);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float v = fmaf(rb[min(max(qpos[mt] - (pre ? 0 : np) - (j0 + 16 * a + 4 * g + r), 0), p.nrel - 1)], CA_LOG2E, sc[mt][a][r]);
-                            sc[mt][a][r] = v < CA_LOWEST ? CA_LOWEST : v;          // (the lowest value times log2 e is no longer finite)
+                            for (int r = 0; r < 4; ++r) sc[mt][a][r] = fmaf(sc[mt][a][r], ksc[a][r], end);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float bias = rb[min(max(qpos[mt] - kpos0 - (j0 + 16 * a + 4 * g + r), 0), p.nrel - 1)];
+                                sc[mt][a][r] = fmaf(sc[mt][a][r], ksc[a][r], ca_bias2(bias));
+                            }
                         }
-                    }
+                    } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (j0 + 16 * a + 4 * g + r >= lim[mt]) sc[mt][a][r] = -INFINITY;
+                        for (int r = 0; r < 4; ++r) sc[mt][a][r] *= ksc[a][r];
+                    }
+                    if (masked)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (j0 + 16 * a + 4 * g + r >= lim[mt]) sc[mt][a][r] = -INFINITY;
                 }
             }
             if (masked || p.rel_bias)

@@ -228,6 +228,54 @@ __device__ __forceinline__ VfBest vf_wave_best(VfBest a) {
     for (int o = 32; o > 0; o >>= 1) vf_better(a, __shfl_xor(a.v, o, 64), __shfl_xor(a.i, o, 64));
     return a;
 }
+// The best of lo .. hi - 1 of a row by one wave, eight loads on the way (a lane's indices ascend: the first of equals stays)
+__device__ __forceinline__ VfBest vf_wave_argmax(const float* row, int lo, int hi) {
+    VfBest a = {-INFINITY, 0x7fffffff};
+    int j = lo + 4 * (threadIdx.x & 63);
+    for (; j + 7 * 256 + 4 <= hi; j += 8 * 256) {
+        VfF4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const VfF4*>(row + j + 256 * u);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (x[u].v[e] > a.v) { a.v = x[u].v[e]; a.i = j + 256 * u + e; }
+    }
+    for (; j < hi; j += 256)
+        for (int e = 0; e < 4; ++e)
+            if (j + e < hi && row[j + e] > a.v) { a.v = row[j + e]; a.i = j + e; }
+    return vf_wave_best(a);
+}
+// All rows of one batch entry in one workgroup: each of the n + 1 rows by 16 / (n + 1) waves (more than 16 rows: one wave each, in turns)
+__global__ __launch_bounds__(1024) void verify_greedy_row_kernel(SmxVerifyParams p) {
+    __shared__ VfBest sh[VF_MAXN + 1][VF_WAVES];
+    const int b = blockIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63, rows = p.n + 1;
+    const int parts = rows > VF_WAVES ? 1 : VF_WAVES / rows, len = ((p.V + parts - 1) / parts + 3) & ~3;
+    const long long id = lane < p.n ? p.ids[b * p.ids_bs + lane] : -1;
+    for (int k = w; k < rows * parts; k += VF_WAVES) {
+        const int i = k % rows, part = k / rows;
+        const VfBest a = vf_wave_argmax(p.target + b * p.t_bs + i * p.t_ts, min(part * len, p.V), min((part + 1) * len, p.V));
+        if (lane == 0) sh[i][part] = a;
+    }
+    __syncthreads();
+    if (w) return;
+    int best = 0, last = 0;                           // of row `lane`, and of row n (64 drafts: the 65th row)
+    for (int r = 0; r < 2; ++r) {
+        const int i = r ? p.n : min(lane, p.n);
+        VfBest a = sh[i][0];
+        for (int q = 1; q < parts; ++q) vf_better(a, sh[i][q].v, sh[i][q].i);
+        (r ? last : best) = a.i == 0x7fffffff ? 0 : a.i;              // (nothing above -inf)
+    }
+    const unsigned long long no = ~__ballot(lane < p.n && id == best);
+    const int r = no ? min(__ffsll((long long)no) - 1, p.n) : p.n;
+    const int tok = __shfl(best, min(r, 63), 64);
+    if (lane == 0) {
+        p.accepted[b] = r;
+        p.token[b] = r < p.n ? tok : last;
+    }
+}
+// Long rows: a workgroup per row, then a second launch
 __global__ __launch_bounds__(1024) void verify_best_kernel(SmxVerifyParams p, VfBest* best) {
     __shared__ VfBest sh[VF_WAVES];
     const int i = blockIdx.x, b = blockIdx.y;
@@ -285,9 +333,13 @@ static int vf_pieces(const SmxVerifyParams& p) {
     return c < 2 ? 1 : c > VF_MAXC ? VF_MAXC : c;
 }
 
+// One launch for the greedy form where a workgroup gets through its rows in the time of the second launch: it reads 100 GB/s (1 row set of 5 x
+// 32 128: 8 us, in two launches 5.7 + 1.9 and 3 us of host time; 64 x 5 x 50 265: 10 against 15 + 4; 5 x 250 027: 12 + 2 in two).
+static bool vf_greedy_one(const SmxVerifyParams& p) { return (long long)(p.n + 1) * p.V <= 400000; }
+
 extern "C" long long smx_verify_draft_ws_bytes(const SmxVerifyParams* p) {
     if (vf_check(*p)) return SMX_EINVAL;
-    if (!p->u) return 8ll * p->B * (p->n + 1);
+    if (!p->u) return vf_greedy_one(*p) ? 0 : 8ll * p->B * (p->n + 1);
     const int c = vf_pieces(*p);
     return c == 1 ? 0 : 8ll * p->B * c * VF_WAVES;
 }
@@ -306,6 +358,8 @@ extern "C" int smx_verify_draft(const SmxVerifyParams* pp, hipStream_t stream) {
             hipLaunchKernelGGL(verify_sums_kernel, dim3(c, p.B), dim3(1024), 0, stream, p, len, (double*)p.ws);
             hipLaunchKernelGGL(verify_pick_kernel, dim3(p.B), dim3(1024), 0, stream, p, S, len, (double*)p.ws);
         }
+    } else if (vf_greedy_one(p)) {
+        hipLaunchKernelGGL(verify_greedy_row_kernel, dim3(p.B), dim3(1024), 0, stream, p);
     } else {
         hipLaunchKernelGGL(verify_best_kernel, dim3(p.n + 1, p.B), dim3(1024), 0, stream, p, (VfBest*)p.ws);
         hipLaunchKernelGGL(verify_greedy_kernel, dim3(p.B), dim3(64), 0, stream, p, (const VfBest*)p.ws);

@@ -62,7 +62,9 @@ class CachedDecoder:
         self.graphs, self.warm = {}, set()
         self.rel = None
         if self.t5:            # row `capacity - 1` of the bias sees every distance: [H, capacity], indexed by query - key
-            self.rel = eng._t5_bias("decoder", capacity, capacity)[0][:, capacity - 1].flip(-1).contiguous()
+            rel = eng._t5_bias("decoder", capacity, capacity)[0][:, capacity - 1].flip(-1)
+            # (the last bucket holds every distance from relative_attention_max_distance on: the operator clamps to the table's end)
+            self.rel = rel[:, :min(capacity, lc.relative_attention_max_distance + 1)].contiguous()
         else:
             self.max_pos = st.offsets[self.pd + "embed_positions.weight"][2][0] - 1
         self.own = [ops.KVCache.empty(self.N, self.H, capacity, self.hd, self.fmt, eng.dev) for _ in self.names]

@@ -192,6 +192,33 @@ def test_attention_distance_bias(fmt, dtype, D):
         _check(q, c, [4, 150, 2], rel=rel, pre=pre, plen=[45])
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 16])
+def test_attention_bias_that_masks(fmt, D):
+    """Distances masked with the type's lowest value or with -inf count as nothing next to others; where every key has the lowest value, all count
+    alike (the scores vanish beside it); where every key has -inf, nothing is seen."""
+    from speechmix_amd import ops
+    c = _filled(2, 2, 100, D, fmt, 35)
+    q = torch.randn(2, 1, 2, D, device="cuda", generator=_gen(36)).to(torch.bfloat16)
+    kl = torch.tensor([100, 37], dtype=torch.int32, device="cuda")
+    low = torch.finfo(torch.float32).min
+    for m in (low, -float("inf")):
+        rel = torch.full((2, 101), m, device="cuda")
+        rel[:, :5] = 0.25                              # the last five keys are seen
+        o, lse = ops.attention_cached(q, c, kl, rel_bias=rel, want_lse=True)
+        for b, n in enumerate((100, 37)):
+            K, V = (R.values(t[b:b + 1, :, n - 5:n], s[b:b + 1, :, n - 5:n] if s is not None else None, fmt) for t, s in ((c.k, c.ks), (c.v, c.vs)))
+            ref = R.attention(q[b:b + 1], K, V, [5], None, None, None, 1, True, D ** -0.5, torch.full((2, 5), 0.25))
+            tol_o, tol_l = R.attention_bounds(*ref, D, q.dtype)
+            assert ((o[b:b + 1].double().cpu() - ref[0]).abs() <= tol_o).all() and ((lse[b:b + 1].double().cpu() - ref[1]).abs() <= tol_l).all()
+        o, lse = ops.attention_cached(q, c, kl, rel_bias=torch.full((2, 7), m, device="cuda"), want_lse=True)
+        if m == low:
+            flat, _ = ops.attention_cached(torch.zeros_like(q), c, kl)
+            assert (o.double() - flat.double()).abs().max() <= 2.0 ** -7 * flat.double().abs().max() and (lse == low).all()
+        else:
+            assert (o == 0).all() and (lse == m).all()
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("NG,R_,H,Hkv,D,P,Tq", [(1, 2, 2, 2, 64, 100, 1), (2, 3, 4, 2, 128, 65, 2), (3, 8, 2, 2, 64, 33, 1), (1, 33, 4, 1, 64, 70, 1),
@@ -326,7 +353,7 @@ def _verify(p, ids, q, u):
 
 
 @pytest.mark.parametrize("mode", ["sampled", "picked", "greedy"])
-@pytest.mark.parametrize("B,n,V", [(1, 0, 1), (5, 0, 2048), (3, 1, 2047), (4, 4, 2049), (16, 7, 50265), (2, 64, 300), (40, 3, 5), (300, 2, 4097), (1, 4, 32128)])
+@pytest.mark.parametrize("B,n,V", [(1, 0, 1), (5, 0, 2048), (3, 1, 2047), (4, 4, 2049), (16, 7, 50265), (2, 64, 300), (40, 3, 5), (300, 2, 4097), (1, 4, 32128), (2, 15, 9000), (2, 16, 9001), (2, 3, 250027)])
 def test_verify(mode, B, n, V):
     p, q, ids, u = _probs(B, n, V, B + V)
     if mode == "greedy":

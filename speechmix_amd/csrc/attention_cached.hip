@@ -105,32 +105,58 @@ static bool ca_mfma_ok(const SmxCachedAttnParams& p) {
     return true;
 }
 static int ca_cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
-// Splits of `cap` keys for `base` workgroups: up to `want` workgroups.  A split costs the second launch (5 us) and its partial rows, so it has to take
-// at least 512 keys, and 2 048 where the rows alone already give the chip a workgroup per CU (32 x 16 heads x 777 keys: one launch 13 us,
+#define CA_SHORT 256          // keys of a cache that one wave takes
+// Splits of `cap` keys for `base` workgroups: up to `want` workgroups.  A split costs the second launch (4 us) and its partial rows, so it has to take
+// at least 512 keys (256 where few workgroups share the chip), and 2 048 where the rows alone already give it a workgroup per CU (32 x 16 heads x 777 keys: one launch 13 us,
 // two splits 14 + 4; 16 x 16 heads x 8 192 int8 keys: 84 us unsplit, 52 in four).
 static int ca_splits(long long base, int cap, long long want) {
-    const long long n = want / base, most = ca_cdiv(cap, base >= 256 ? 2048 : 512);
+    const long long n = want / base, most = ca_cdiv(cap, base >= 256 ? 2048 : base >= 64 ? 512 : 256);
     const long long m = n < most ? n : most;
     return (int)(m < 1 ? 1 : m > 64 ? 64 : m);
+}
+static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, CaPlan& pl, long long& items) {
+    const SmxKVCache& m = p.own.k ? p.own : p.pre;
+    const long long ro = p.own.k ? (long long)p.Tq * pl.G : 0, rp = p.pre.k ? (long long)pl.R * p.Tq * pl.G : 0;
+    pl.mbo = ca_cdiv(ro, 16 * mt);
+    pl.mbp = ca_cdiv(rp, 16 * mt);
+    const long long bo = (long long)pl.mbo * p.own.B * pl.Hkv, bp = (long long)pl.mbp * p.pre.B * pl.Hkv;
+    // what is resident at once: four workgroups per CU of the small form, two or three of the others; a prefix gets what its rows' own keys leave
+    const long long want = mt == 1 && m.D == 64 ? 1024 : 512;
+    // a wave per item where there are many items of few keys: a workgroup's other three waves would have nothing to do (16 384 rows and heads of
+    // 43 keys behind prefixes: FIG_S4 us with a workgroup each, FIG_S1 so)
+    pl.single = p.own.k && ro <= 16 && p.own.cap <= CA_SHORT && bo > 512;
+    pl.nso = !p.own.k ? 0 : pl.single ? 1 : ca_splits(bo, p.own.cap, want);
+    const long long left = want - (pl.single ? 0 : bo * pl.nso);        // (those of short caches are soon gone)
+    pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, left > want / 2 ? left : want / 2) : 0;
+    pl.items_p = (int)(bp * pl.nsp);
+    pl.items_o = (int)(bo * pl.nso);
+    items = bp * pl.nsp + bo * pl.nso;
+    pl.join = pl.nso + pl.nsp > 1;
+}
+static CaDiv ca_divisor(int d) {
+    CaDiv v = {0u, 0, d};
+    while ((1ll << v.k) < d) ++v.k;
+    v.m = (unsigned)(((1ull << (31 + v.k)) + d - 1) / d);
+    return v;
 }
 static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long long& items) {
     const SmxKVCache& m = p.own.k ? p.own : p.pre;
     pl.Hkv = m.H;
     pl.G = p.H / m.H;
     pl.R = p.pre.k ? p.B / p.pre.B : 1;
+    pl.per = ca_divisor(p.Tq * pl.G);
+    pl.g = ca_divisor(pl.G);
     const long long ro = p.own.k ? (long long)p.Tq * pl.G : 0, rp = p.pre.k ? (long long)pl.R * p.Tq * pl.G : 0, rmax = ro > rp ? ro : rp;
-    const int mt = dtype == SMX_F32 || rmax <= 16 ? 1 : rmax <= 32 || m.D == 128 ? 2 : 4;
-    pl.mbo = ca_cdiv(ro, 16 * mt);
-    pl.mbp = ca_cdiv(rp, 16 * mt);
-    const long long bo = (long long)pl.mbo * p.own.B * pl.Hkv, bp = (long long)pl.mbp * p.pre.B * pl.Hkv;
-    // what is resident at once: four workgroups per CU of the small form, two or three of the others; a prefix gets what its rows' own keys leave
-    const long long want = mt == 1 && m.D == 64 ? 1024 : 512;
-    pl.nso = p.own.k ? ca_splits(bo, p.own.cap, want) : 0;
-    const long long left = want - bo * pl.nso;
-    pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, left > want / 2 ? left : want / 2) : 0;
-    pl.items_p = (int)(bp * pl.nsp);
-    items = bp * pl.nsp + bo * pl.nso;
-    pl.join = pl.nso + pl.nsp > 1;
+    int mt = dtype == SMX_F32 || rmax <= 16 ? 1 : rmax <= 32 || m.D == 128 ? 2 : 4;
+    // (own keys that outweigh the prefix's decide: more of their small items are resident beside a small form)
+    if (p.own.k && p.pre.k && ro <= 16 && (long long)p.own.B * p.own.cap > (rp + 15) / 16 * p.pre.B * (long long)p.pre.cap) mt = 1;
+    ca_plan_mt(p, mt, pl, items);
+    // Fewer rows per item while that leaves CUs idle: a block of keys takes 2.5 us for 64 rows and 0.9 for 16 (33 rows x 171 keys x 12 heads: 15.9 us
+    // in 12 workgroups, FIG_MT in 36).
+    while (mt > 1 && items < 256) {
+        mt >>= 1;
+        ca_plan_mt(p, mt, pl, items);
+    }
     return mt;
 }
 
@@ -150,17 +176,41 @@ extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp
         if (dtype == SMX_BF16) hipLaunchKernelGGL((attn_cached_simple<FMT, bf16_t>), dim3(n), dim3(256), 0, stream, p);               \
         else hipLaunchKernelGGL((attn_cached_simple<FMT, float>), dim3(n), dim3(256), 0, stream, p);                                  \
     } while (0)
-#define CA_MFMA_D(FMT, D)                                                                                                             \
-    do {                                                                                                                              \
-        if (dtype == SMX_F32) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 1, float>), grid, dim3(256), 0, stream, p, pl);            \
-        else if (mt == 1) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 1, bf16_t>), grid, dim3(256), 0, stream, p, pl);               \
-        else if (mt == 2) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, 2, bf16_t>), grid, dim3(256), 0, stream, p, pl);               \
-        else hipLaunchKernelGGL((attn_cached_mfma<FMT, D, D == 64 ? 4 : 2, bf16_t>), grid, dim3(256), 0, stream, p, pl);              \
+#define CA_GO(FMT, D, MT, MODE, T) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, MT, MODE, T>), grid, dim3(256), 0, stream, p, pl)
+#define CA_MODE1(FMT, D, T)                                           \
+    do {                                                              \
+        if (mode == CA_SINGLE) CA_GO(FMT, D, 1, CA_SINGLE, T);        \
+        else if (mode == CA_MIXED) CA_GO(FMT, D, 1, CA_MIXED, T);     \
+        else CA_GO(FMT, D, 1, CA_PLAIN, T);                           \
+    } while (0)
+#define CA_MODEN(FMT, D, MT, T)                                       \
+    do {                                                              \
+        if (mode == CA_SMALL) CA_GO(FMT, D, MT, CA_SMALL, T);         \
+        else if (mode == CA_MIXED) CA_GO(FMT, D, MT, CA_MIXED, T);    \
+        else CA_GO(FMT, D, MT, CA_PLAIN, T);                          \
+    } while (0)
+#define CA_MFMA_D(FMT, D)                                             \
+    do {                                                              \
+        if (dtype == SMX_F32) CA_MODE1(FMT, D, float);                \
+        else if (mt == 1) CA_MODE1(FMT, D, bf16_t);                   \
+        else if (mt == 2) CA_MODEN(FMT, D, 2, bf16_t);                \
+        else CA_MODEN(FMT, D, (D == 64 ? 4 : 2), bf16_t);             \
     } while (0)
 #define CA_MFMA(FMT)                           \
     do {                                       \
         if (D == 64) CA_MFMA_D(FMT, 64);       \
         else CA_MFMA_D(FMT, 128);              \
+    } while (0)
+
+#define CA_JOIN_T(D, T)                                                                                                               \
+    do {                                                                                                                              \
+        if (wide) hipLaunchKernelGGL((attn_cached_join<D, 4, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                          \
+        else hipLaunchKernelGGL((attn_cached_join<D, 1, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                               \
+    } while (0)
+#define CA_JOIN(D)                                 \
+    do {                                           \
+        if (dtype == SMX_F32) CA_JOIN_T(D, float); \
+        else CA_JOIN_T(D, bf16_t);                 \
     } while (0)
 
 extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hipStream_t stream) {
@@ -180,19 +230,19 @@ extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hi
             pl.po = (float*)p.ws;
             pl.pml = pl.po + rows * D;
         }
-        const dim3 grid((unsigned)items);
+        const bool few = p.own.k && p.pre.k && (long long)p.Tq * pl.G <= 16;
+        const int mode = pl.single ? (p.pre.k ? CA_MIXED : CA_SINGLE) : mt > 1 && few ? CA_SMALL : CA_PLAIN;
+        const dim3 grid((unsigned)(pl.items_p + (pl.single ? (pl.items_o + 3) / 4 : pl.items_o)));
         if (fmt == SMX_KV_E4M3) CA_MFMA(SMX_KV_E4M3);
         else if (fmt == SMX_KV_INT8) CA_MFMA(SMX_KV_INT8);
         else CA_MFMA(SMX_KV_BF16);
         if (pl.join) {
-            const dim3 jg((unsigned)(((long long)p.B * p.H * p.Tq + 3) / 4));
-            if (D == 64) {
-                if (dtype == SMX_F32) hipLaunchKernelGGL((attn_cached_join<64, float>), jg, dim3(256), 0, stream, p, pl, 16 * mt);
-                else hipLaunchKernelGGL((attn_cached_join<64, bf16_t>), jg, dim3(256), 0, stream, p, pl, 16 * mt);
-            } else {
-                if (dtype == SMX_F32) hipLaunchKernelGGL((attn_cached_join<128, float>), jg, dim3(256), 0, stream, p, pl, 16 * mt);
-                else hipLaunchKernelGGL((attn_cached_join<128, bf16_t>), jg, dim3(256), 0, stream, p, pl, 16 * mt);
-            }
+            const long long rows = (long long)p.B * p.H * p.Tq;
+            // a workgroup per row where there are many splits to add (32 splits of 128 wide: FIG_J1 us by a wave, FIG_J4 by four)
+            const bool wide = pl.nso > 8 || pl.nsp > 8;
+            const dim3 jg((unsigned)(wide ? rows : (rows + 3) / 4));
+            if (D == 64) CA_JOIN(64);
+            else CA_JOIN(128);
         }
     } else {
         switch (fmt) {

@@ -34,11 +34,20 @@ constexpr int ca_occ(int es, int d, int mt, int qsize) { return qsize == 4 || (e
 // blocks on the way at once
 constexpr int ca_depth(int es, int d, int mt, int qsize) { return CA_PF; }
 
+// Division of 0 <= r < 2^31 by a number known to the host: k = ceil(log2 d), m = ceil(2^(31 + k) / d) < 2^32, and 2 r m / 2^(32 + k) falls short of
+// nothing, since m d - 2^(31 + k) < 2^k.  (The compiler's division is some thirty instructions, a few of them per row: a cold kernel waits for
+// every line of its code.)
+struct CaDiv { unsigned m; int k, d; };
+__device__ __forceinline__ int ca_div(const CaDiv& v, int r) { return (int)(__umulhi((unsigned)r << 1, v.m) >> v.k); }
+
 struct CaPlan {
+    CaDiv per, g;                 // by Tq * G, by G
     int G, Hkv, R;                // query heads per KV head; rows per prefix
     int mbo, mbp;                 // blocks of 16 * MT rows per (entry, KV head): own, prefix
     int nso, nsp;                 // key splits: own, prefix
-    int items_p;                  // workgroups of the prefix part (they come first)
+    int items_p;                  // work items = workgroups of the prefix part (they come first)
+    int items_o;                  // work items of the own part
+    int single;                   // own part: a wave per item, four items per workgroup (short caches, many rows)
     int join;                     // partial results to po / pml instead of the output
     float *po, *pml;              // [item][16 MT][D], [item][16 MT][2]
 };
@@ -180,10 +189,10 @@ template <int D> struct CaShared {       // where the four waves meet
     float m[CA_WAVES][16], l[CA_WAVES][16];
     __attribute__((aligned(16))) float o[CA_WAVES][16][D + 4];
 };
-struct CaItem { bool pre; int s, hk, b, row0; };      // key split, KV head, batch entry, first row
+struct CaItem { bool pre; int s, hk, b, row0; long long slot; };      // key split, KV head, batch entry, first row; number among all items
 
-// One work item: 16 * MT rows (as many as there are of the kernel's 16 * MTB) over one split of the keys
-template <int FMT, int D, int MT, int MTB, typename T>
+// One work item: 16 * MT rows (as many as there are of the kernel's 16 * MTB) over one split of the keys, by the workgroup's WV = 4 waves or by one
+template <int FMT, int D, int MT, int MTB, int WV, typename T>
 __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPlan& pl, const CaItem& it, CaShared<D>& sh) {
     enum { ES = CaFmt<FMT>::ES, NB = (ES * D == 64 && MT <= CA_NB2) ? 2 : 1, PF = ca_depth(CaFmt<FMT>::ES, D, MT, sizeof(T)), BK = 32 * NB, KF = D / 32, DT = D / 16,
            NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2 };
@@ -195,25 +204,25 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
     const int ns = pre ? pl.nsp : pl.nso;
     const int per = p.Tq * pl.G, nrows = (pre ? pl.R : 1) * per, b0 = pre ? b * pl.R : b;
     int np = 0, nk = 0;
-    if (p.pre.k) np = p.plen ? min(max(p.plen[b0 / pl.R], 0), p.pre.cap) : p.pre.cap;
+    if (p.pre.k) np = p.plen ? min(max(p.plen[pre ? b : b / pl.R], 0), p.pre.cap) : p.pre.cap;
     if (p.own.k && !pre) nk = p.klen ? min(max(p.klen[b], 0), p.own.cap) : p.own.cap;
     const bool causal = p.causal && !pre;
     const int rlast = min(nrows, row0 + 16 * MT) - 1;
     // keys that the block's first row sees (all rows see them) and that its last row sees
-    const int nmax = pre ? np : causal ? max(min(nk, nk - p.Tq + rlast / pl.G + 1), 0) : nk;
-    const int nall = causal ? max(nk - p.Tq + row0 / pl.G + 1, 0) : nmax;
+    const int nmax = pre ? np : causal ? max(min(nk, nk - p.Tq + ca_div(pl.g, rlast) + 1), 0) : nk;
+    const int nall = causal ? max(nk - p.Tq + ca_div(pl.g, row0) + 1, 0) : nmax;
     const int nblk = (nmax + BK - 1) / BK, bps = (nblk + ns - 1) / ns;
     const int blk_end = min(nblk, (s + 1) * bps);
     const long long base = (long long)b * c.bs + (long long)hk * c.hs, sbase = (long long)b * c.sbs + (long long)hk * c.shs;
     const CaView cv = {(const char*)c.k + base * ES, (const char*)c.v + base * ES, c.ks + sbase, c.vs + sbase, (int)c.ts * ES, nmax,
                        i * (int)c.ts * ES + 16 * g, 4 * g * (int)c.ts * ES + 4 * Blk::VW * i, 4 * (16 * (i >> 2) + 4 * g + (i & 3))};
     Blk buf[PF];
-    int blk = s * bps + w;
+    int blk = s * bps + (WV == 1 ? 0 : w);
 #pragma unroll
     for (int f = 0; f < PF; ++f)
-        if (blk + CA_WAVES * f < blk_end) {
-            ca_load_k<FMT, D, NB>(buf[f], cv, (blk + CA_WAVES * f) * BK);
-            ca_load_v<FMT, D, NB>(buf[f], cv, (blk + CA_WAVES * f) * BK);
+        if (blk + WV * f < blk_end) {
+            ca_load_k<FMT, D, NB>(buf[f], cv, (blk + WV * f) * BK);
+            ca_load_v<FMT, D, NB>(buf[f], cv, (blk + WV * f) * BK);
         }
     // ---- this lane's rows
     const int kpos0 = pre ? 0 : np;                     // position of key 0
@@ -223,8 +232,8 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int r = row0 + 16 * mt + i;
-        const int rr = min(r, nrows - 1), bb = b0 + rr / per, t = rr % per / pl.G;
-        hq[mt] = hk * pl.G + rr % pl.G;
+        const int rr = min(r, nrows - 1), br = pre ? ca_div(pl.per, rr) : 0, bb = b0 + br, rt = rr - br * per, t = ca_div(pl.g, rt);
+        hq[mt] = hk * pl.G + rt - t * pl.G;
         int own = nk;                                   // (a prefix row's own length: for its position only)
         if (pre) own = !p.own.k ? 0 : p.klen ? min(max(p.klen[bb], 0), p.own.cap) : p.own.cap;
         qpos[mt] = np + own - p.Tq + t;
@@ -233,18 +242,23 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
         for (int f = 0; f < KF; ++f) {
             const int d = ES == 1 ? 64 * (f >> 1) + 16 * g + 8 * (f & 1) : 32 * f + 8 * g;
-            float x[8];
-            load8(q + d, x);
+            if (NQ == 1) {
+                const uint4 u = r < nrows ? *reinterpret_cast<const uint4*>(q + d) : make_uint4(0u, 0u, 0u, 0u);
+                qf[mt][0][f][0] = u.x; qf[mt][0][f][1] = u.y; qf[mt][0][f][2] = u.z; qf[mt][0][f][3] = u.w;
+            } else {
+                float x[8];
+                load8(q + d, x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float u = r < nrows ? x[2 * e] : 0.f, v = r < nrows ? x[2 * e + 1] : 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    float u = r < nrows ? x[2 * e] : 0.f, v = r < nrows ? x[2 * e + 1] : 0.f;
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) {          // the part of the value that n earlier bf16 numbers leave over
-                    const unsigned h = pack_bf2(u, v);
-                    qf[mt][n][f][e] = h;
-                    // (the first part of an infinity or NaN holds it all)
-                    u = n == 0 && !(fabsf(u) < INFINITY) ? 0.f : u - __uint_as_float(h << 16);
-                    v = n == 0 && !(fabsf(v) < INFINITY) ? 0.f : v - __uint_as_float(h & 0xffff0000u);
+                    for (int n = 0; n < NQ; ++n) {      // the part of the value that n earlier bf16 numbers leave over
+                        const unsigned h = pack_bf2(u, v);
+                        qf[mt][n][f][e] = h;
+                        // (the first part of an infinity or NaN holds it all)
+                        u = n == 0 && !(fabsf(u) < INFINITY) ? 0.f : u - __uint_as_float(h << 16);
+                        v = n == 0 && !(fabsf(v) < INFINITY) ? 0.f : v - __uint_as_float(h & 0xffff0000u);
+                    }
                 }
             }
         }
@@ -262,7 +276,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
     }
     auto block = [&](Blk& x) {
         const int j0 = blk * BK;
-        const bool more = blk + PF * CA_WAVES < blk_end;
+        const bool more = blk + PF * WV < blk_end;
         const bool masked = j0 + BK > nall;
         // ---- scores
         f32x4_t sc[MT][2 * NB];                         // q . codes; times ksc it is the score in log 2 units
@@ -319,7 +333,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
                 for (int r = 0; r < 4; ++r) ksc[a][r] = 1.f;
         }
-        if (more) ca_load_k<FMT, D, NB>(x, cv, j0 + PF * CA_WAVES * BK);
+        if (more) ca_load_k<FMT, D, NB>(x, cv, j0 + PF * WV * BK);
         bool odd = false;                               // bf16: a value that is not finite in a block of which some row must not see all
         if (FMT == SMX_KV_BF16 && masked) {
             bool bad = false;
@@ -447,8 +461,8 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                 }
             }
         }
-        if (more) ca_load_v<FMT, D, NB>(x, cv, j0 + PF * CA_WAVES * BK);
-        blk += CA_WAVES;
+        if (more) ca_load_v<FMT, D, NB>(x, cv, j0 + PF * WV * BK);
+        blk += WV;
     };
     while (blk < blk_end) {
 #pragma unroll
@@ -456,6 +470,35 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             if (f == 0 || blk < blk_end) block(buf[f]);
     }
 
+    if (WV == 1) {                                      // a wave has all of its rows: out of the registers
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float L = l[mt];
+            L += __shfl_xor(L, 16, 64);
+            L += __shfl_xor(L, 32, 64);
+            const int r = row0 + 16 * mt + i;
+            if (r >= nrows) continue;
+            if (pl.join) {
+                const long long pr = it.slot * (16 * MTB) + 16 * mt + i;
+                if (g == 0) *reinterpret_cast<float2*>(pl.pml + 2 * pr) = make_float2(m[mt], L);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int d = 0; d < DT; d += 4)
+                        *reinterpret_cast<float4*>(pl.po + pr * D + DT * (4 * g + q) + d) = make_float4(acc[mt][d][q], acc[mt][d + 1][q], acc[mt][d + 2][q], acc[mt][d + 3][q]);
+            } else {
+                const int br = pre ? ca_div(pl.per, r) : 0, bb = b0 + br, rt = r - br * per, t = ca_div(pl.g, rt), h = hk * pl.G + rt - t * pl.G;
+                const float inv = 1.f / L;
+                T* out = reinterpret_cast<T*>(p.o) + bb * p.o_bs + t * p.o_ts + h * p.o_hs;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) Cvt<T>::st(out + DT * (4 * g + q) + d, L == 0.f ? 0.f : acc[mt][d][q] * inv);
+                if (p.lse && g == 0) p.lse[((long long)bb * p.H + h) * p.Tq + t] = ca_lse(m[mt], L);
+            }
+        }
+        return;
+    }
     // ---- the four waves meet: rows of 16, one tile at a time
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -487,7 +530,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             for (int d = 0; d < DT; ++d) o[d] = fmaf(sh.o[v][row][d0 + d], f, o[d]);
         }
         if (pl.join) {
-            const long long pr = (long long)blockIdx.x * (16 * MTB) + 16 * mt + row;
+            const long long pr = it.slot * (16 * MTB) + 16 * mt + row;
             if (r < nrows) {
                 if (d0 == 0) {
                     pl.pml[2 * pr] = M;
@@ -497,7 +540,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                 for (int d = 0; d < DT; d += 4) *reinterpret_cast<float4*>(pl.po + pr * D + d0 + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
             }
         } else if (r < nrows) {
-            const int bb = b0 + r / per, t = r % per / pl.G, h = hk * pl.G + r % pl.G;
+            const int br = pre ? ca_div(pl.per, r) : 0, bb = b0 + br, rt = r - br * per, t = ca_div(pl.g, rt), h = hk * pl.G + rt - t * pl.G;
             const float inv = L == 0.f ? 0.f : 1.f / L;
             T* out = reinterpret_cast<T*>(p.o) + bb * p.o_bs + t * p.o_ts + h * p.o_hs + d0;
 #pragma unroll
@@ -507,36 +550,48 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
     }
 }
 
-template <int FMT, int D, int MT, typename T>
+// What a launch's items look like.  Each combination is a kernel of its own: a second body beside the one that runs costs 1.4 us a launch (its
+// instructions lie between those that run), as much as a short cache takes.
+enum {
+    CA_PLAIN = 0,       // every item: 16 * MT rows by four waves
+    CA_SINGLE = 1,      // own keys only, an item per wave
+    CA_SMALL = 2,       // prefix items as in CA_PLAIN, own items of up to 16 rows by four waves
+    CA_MIXED = 3        // prefix items as in CA_PLAIN, own items by a wave each
+};
+template <int FMT, int D, int MT, int MODE, typename T>
 __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void attn_cached_mfma(SmxCachedAttnParams p, CaPlan pl) {
     __shared__ CaShared<D> sh;
-    int id = blockIdx.x;
     CaItem it;
-    it.pre = id < pl.items_p;
-    if (!it.pre) id -= pl.items_p;
-    const int ns = it.pre ? pl.nsp : pl.nso, cb = it.pre ? p.pre.B : p.own.B, per = p.Tq * pl.G, nrows = it.pre ? pl.R * per : per;
+    it.pre = MODE != CA_SINGLE && blockIdx.x < (unsigned)pl.items_p;
+    const bool single = MODE == CA_SINGLE || (MODE == CA_MIXED && !it.pre);
+    int id = it.pre ? blockIdx.x : blockIdx.x - pl.items_p;
+    if (single) id = 4 * id + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (single && id >= pl.items_o) return;             // (the last workgroup's spare waves; no barrier in that form)
+    it.slot = (it.pre ? 0 : pl.items_p) + (long long)id;
+    const int ns = it.pre ? pl.nsp : pl.nso, cb = it.pre ? p.pre.B : p.own.B;
     it.s = id % ns;
     id /= ns;
     it.hk = id % pl.Hkv;
     id /= pl.Hkv;
     it.b = id % cb;
     it.row0 = id / cb * (16 * MT);
-    // (a batch behind a prefix: the prefix's many rows choose MT, a row's own keys have few)
-    if (MT > 1 && nrows - it.row0 <= 16) ca_body<FMT, D, 1, MT, T>(p, pl, it, sh);
-    else ca_body<FMT, D, MT, MT, T>(p, pl, it, sh);
+    if (MODE == CA_SINGLE) ca_body<FMT, D, 1, MT, 1, T>(p, pl, it, sh);
+    else if (MODE == CA_MIXED && !it.pre) ca_body<FMT, D, 1, MT, 1, T>(p, pl, it, sh);
+    else if (MODE == CA_SMALL && !it.pre) ca_body<FMT, D, 1, MT, 4, T>(p, pl, it, sh);
+    else ca_body<FMT, D, MT, MT, 4, T>(p, pl, it, sh);
 }
 
-// O = sum over the splits of both parts, in order.  One wave per (row, head, query).
-template <int D, typename T>
+// O = sum over the splits of both parts, in a fixed order: JW waves per (row, head, query), D / 4 lanes per split.  A lane's loads depend on nothing but
+// the weights, and with four waves even 64 splits are four (D = 128: eight) of them.
+template <int D, int JW, typename T>
 __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, CaPlan pl, int mt16) {
-    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    enum { LD = D / 4, NG = 64 / LD * JW };
+    const int lane = threadIdx.x & 63, tid = JW == 4 ? threadIdx.x : lane;
+    const long long id = JW == 4 ? (long long)blockIdx.x : (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= (long long)p.B * p.H * p.Tq) return;
     const int t = (int)(id % p.Tq), h = (int)(id / p.Tq % p.H), b = (int)(id / ((long long)p.Tq * p.H)), hk = h / pl.G;
-    // a lane holds four elements of every NG-th split: its loads depend on nothing but the weights
-    enum { LD = D / 4, NG = 64 / LD };
-    const int grp = lane / LD, dl = lane % LD * 4;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    const int grp = tid / LD, dl = tid % LD * 4;
+    float m = CA_LOWEST, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int part = 0; part < 2; ++part) {
         const SmxKVCache& c = part ? p.own : p.pre;
         if (!c.k) continue;
@@ -546,7 +601,7 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
         const float* po = pl.po + (it * mt16 + r % mt16) * D + dl;
         const long long step = (long long)mt16 * D;
         // at most 64 splits: a lane holds one's maximum and sum
-        float ms = -INFINITY, ls = 0.f;
+        float ms = CA_LOWEST, ls = 0.f;
         if (lane < ns) {
             const float2 q = *reinterpret_cast<const float2*>(pl.pml + 2 * ((it + lane) * mt16 + r % mt16));
             ms = q.x;
@@ -577,11 +632,18 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
     for (int k = LD; k < 64; k <<= 1)
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] += __shfl_xor(o[d], k, 64);
+    if (JW == 4) {
+        __shared__ __attribute__((aligned(16))) float so[JW][D];
+        if (lane < LD) *reinterpret_cast<float4*>(&so[threadIdx.x >> 6][dl]) = make_float4(o[0], o[1], o[2], o[3]);
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] = (so[0][dl + d] + so[1][dl + d]) + (so[2][dl + d] + so[3][dl + d]);
+    }
     if (grp == 0) {
         T* out = reinterpret_cast<T*>(p.o) + b * p.o_bs + t * p.o_ts + h * p.o_hs + dl;
         const float inv = 1.f / l;
 #pragma unroll
         for (int d = 0; d < 4; ++d) Cvt<T>::st(out + d, l == 0.f ? 0.f : o[d] * inv);
+        if (p.lse && dl == 0) p.lse[id] = ca_lse(m, l);
     }
-    if (p.lse && lane == 0) p.lse[id] = ca_lse(m, l);
 }

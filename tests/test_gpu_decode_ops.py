@@ -235,6 +235,20 @@ def test_attention_shared_prefix(fmt, dtype, NG, R_, H, Hkv, D, P, Tq):
     _check(q, c, klen, pre=pre, plen=plen)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "bf16"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,Tq", [(64, 1), (128, 2)])
+def test_attention_many_short_rows(fmt, dtype, D, Tq):
+    """More rows and heads than the chip holds workgroups, few keys each, alone and behind a prefix."""
+    B, H = 93, 6
+    klen = [(11 * b) % 48 for b in range(B)]
+    c = _filled(B, H, 47, D, fmt, 45)
+    q = torch.randn(B, Tq, H, D, device="cuda", generator=_gen(46)).to(dtype)
+    _check(q, c, klen)
+    pre = _filled(3, H, 20, D, fmt, 47)
+    _check(q, c, klen, pre=pre, plen=[20, 0, 7])
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_long_cache_is_split_and_joined(fmt, dtype):

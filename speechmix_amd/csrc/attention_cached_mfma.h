@@ -14,25 +14,14 @@
 #include "kv_common.h"
 
 #define CA_WAVES 4
-#ifndef CA_OCC
-#define CA_OCC 4
-#endif
-#ifndef CA_PF
-#define CA_PF 1
-#endif
-#ifndef CA_NB2
-#define CA_NB2 0
-#endif
+#define CA_BK 32                  // keys per block and wave (64: more registers than they save instructions; two blocks ahead: spills)
 #define CA_LOG2E 1.44269504088896340736f
 #define CA_LN2 0.69314718055994530942f
 #define CA_BIG 65536.f            // a score may pass the reference by this factor before it moves
 #define CA_LOWEST (-3.402823466e38f)
 
 // waves per SIMD the registers are held to
-constexpr int ca_occ(int es, int d, int mt, int qsize) { return qsize == 4 || (es == 2 && d == 128) || mt > 2 || (mt == 2 && d == 128) ? 2 : mt == 2 || d == 128 ? 3 : CA_OCC; }
-
-// blocks on the way at once
-constexpr int ca_depth(int es, int d, int mt, int qsize) { return CA_PF; }
+constexpr int ca_occ(int es, int d, int mt, int qsize) { return qsize == 4 || (es == 2 && d == 128) || mt > 2 || (mt == 2 && d == 128) ? 2 : mt == 2 || d == 128 ? 3 : 4; }
 
 // Division of 0 <= r < 2^31 by a number known to the host: k = ceil(log2 d), m = ceil(2^(31 + k) / d) < 2^32, and 2 r m / 2^(32 + k) falls short of
 // nothing, since m d - 2^(31 + k) < 2^k.  (The compiler's division is some thirty instructions, a few of them per row: a cold kernel waits for
@@ -100,12 +89,12 @@ typedef __attribute__((ext_vector_type(2))) unsigned ca_u2;
 // One wave's block of BK keys in flight.  K (with its scales) is asked for again as soon as the scores are out, V as soon as the second product is:
 // each is on its way while the other is worked on, out of one set of registers.  All loads go through buffer descriptors that end behind the
 // last visible key: what lies past it comes back as zeros, and there is one code path for whole and partial blocks.
-template <int FMT, int D, int NB>
+template <int FMT, int D>
 struct CaBlock {
     enum { ES = CaFmt<FMT>::ES, KC = D * ES / 64, VW = D * ES / 64 };      // 16-byte K chunks, V registers per key
-    ca_u4 k[2 * NB][KC];
-    unsigned v[2 * NB][4][VW];
-    unsigned ks, vs;        // lane (g, i): the scale of key 16 (i >> 2) + 4 g + (i & 3); DPP row broadcasts hand it to the other lanes of g
+    ca_u4 k[2][KC];
+    unsigned v[2][4][VW];
+    unsigned ks, vs;        // lane (g, i), i < 8: the scale of key 16 (i >> 2) + 4 g + (i & 3); DPP row broadcasts hand it to the other lanes of g
 };
 struct CaView {             // one head of a cache
     const char *k, *v;
@@ -117,31 +106,31 @@ struct CaView {             // one head of a cache
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t ca_rsrc(const void* base, long long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)(bytes < 0x7ffffff0ll ? bytes : 0x7ffffff0ll), 0x00020000);
 }
-template <int FMT, int D, int NB>
+template <int FMT, int D>
 __device__ __forceinline__ unsigned ca_load_scales(const float* s, const CaView& c, int j0) {
     return __builtin_amdgcn_raw_buffer_load_b32(ca_rsrc(s + j0, (c.nmax - j0) * 4ll), c.soff, 0, 0);
 }
-template <int FMT, int D, int NB>
-__device__ __forceinline__ void ca_load_k(CaBlock<FMT, D, NB>& x, const CaView& c, int j0) {
-    typedef CaBlock<FMT, D, NB> B;
+template <int FMT, int D>
+__device__ __forceinline__ void ca_load_k(CaBlock<FMT, D>& x, const CaView& c, int j0) {
+    typedef CaBlock<FMT, D> B;
     int off = c.koff;
     asm volatile("" : "+v"(off));       // (a sum per load: offsets kept from block to block would cost the registers of a tile)
     const __amdgpu_buffer_rsrc_t rs = ca_rsrc(c.k + (long long)j0 * c.tsb, (long long)(c.nmax - 1 - j0) * c.tsb + D * B::ES);
-    if (FMT <= SMX_KV_INT8) x.ks = ca_load_scales<FMT, D, NB>(c.ks, c, j0);
+    if (FMT <= SMX_KV_INT8) x.ks = ca_load_scales<FMT, D>(c.ks, c, j0);
 #pragma unroll
-    for (int a = 0; a < 2 * NB; ++a)
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int q = 0; q < B::KC; ++q) x.k[a][q] = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16 * a * c.tsb + 64 * q, 0, 0);
 }
-template <int FMT, int D, int NB>
-__device__ __forceinline__ void ca_load_v(CaBlock<FMT, D, NB>& x, const CaView& c, int j0) {
-    typedef CaBlock<FMT, D, NB> B;
+template <int FMT, int D>
+__device__ __forceinline__ void ca_load_v(CaBlock<FMT, D>& x, const CaView& c, int j0) {
+    typedef CaBlock<FMT, D> B;
     int off = c.voff;
     asm volatile("" : "+v"(off));
     const __amdgpu_buffer_rsrc_t rs = ca_rsrc(c.v + (long long)j0 * c.tsb, (long long)(c.nmax - 1 - j0) * c.tsb + D * B::ES);
-    if (FMT <= SMX_KV_INT8) x.vs = ca_load_scales<FMT, D, NB>(c.vs, c, j0);
+    if (FMT <= SMX_KV_INT8) x.vs = ca_load_scales<FMT, D>(c.vs, c, j0);
 #pragma unroll
-    for (int a = 0; a < 2 * NB; ++a)
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int o = off + (16 * a + r) * c.tsb;
@@ -185,6 +174,10 @@ __device__ __forceinline__ float ca_scale(unsigned v, int a, int r) {         //
     }
 }
 
+// four outputs side by side (offsets are multiples of 4 elements of a row whose base is 16-byte aligned)
+__device__ __forceinline__ void ca_store4(float* p, const float v[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void ca_store4(bf16_t* p, const float v[4]) { *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])); }
+
 template <int D> struct CaShared {       // where the four waves meet
     float m[CA_WAVES][16], l[CA_WAVES][16];
     __attribute__((aligned(16))) float o[CA_WAVES][16][D + 4];
@@ -194,9 +187,9 @@ struct CaItem { bool pre; int s, hk, b, row0; long long slot; };      // key spl
 // One work item: 16 * MT rows (as many as there are of the kernel's 16 * MTB) over one split of the keys, by the workgroup's WV = 4 waves or by one
 template <int FMT, int D, int MT, int MTB, int WV, typename T>
 __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPlan& pl, const CaItem& it, CaShared<D>& sh) {
-    enum { ES = CaFmt<FMT>::ES, NB = (ES * D == 64 && MT <= CA_NB2) ? 2 : 1, PF = ca_depth(CaFmt<FMT>::ES, D, MT, sizeof(T)), BK = 32 * NB, KF = D / 32, DT = D / 16,
+    enum { ES = CaFmt<FMT>::ES, BK = CA_BK, KF = D / 32, DT = D / 16,
            NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2 };
-    typedef CaBlock<FMT, D, NB> Blk;
+    typedef CaBlock<FMT, D> Blk;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const bool pre = it.pre;
     const int s = it.s, hk = it.hk, b = it.b, row0 = it.row0;
@@ -215,15 +208,13 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
     const int blk_end = min(nblk, (s + 1) * bps);
     const long long base = (long long)b * c.bs + (long long)hk * c.hs, sbase = (long long)b * c.sbs + (long long)hk * c.shs;
     const CaView cv = {(const char*)c.k + base * ES, (const char*)c.v + base * ES, c.ks + sbase, c.vs + sbase, (int)c.ts * ES, nmax,
-                       i * (int)c.ts * ES + 16 * g, 4 * g * (int)c.ts * ES + 4 * Blk::VW * i, 4 * (16 * (i >> 2) + 4 * g + (i & 3))};
-    Blk buf[PF];
+                       i * (int)c.ts * ES + 16 * g, 4 * g * (int)c.ts * ES + 4 * Blk::VW * i, 4 * (16 * ((i >> 2) & 1) + 4 * g + (i & 3))};
+    Blk x;
     int blk = s * bps + (WV == 1 ? 0 : w);
-#pragma unroll
-    for (int f = 0; f < PF; ++f)
-        if (blk + WV * f < blk_end) {
-            ca_load_k<FMT, D, NB>(buf[f], cv, (blk + WV * f) * BK);
-            ca_load_v<FMT, D, NB>(buf[f], cv, (blk + WV * f) * BK);
-        }
+    if (blk < blk_end) {
+        ca_load_k<FMT, D>(x, cv, blk * BK);
+        ca_load_v<FMT, D>(x, cv, blk * BK);
+    }
     // ---- this lane's rows
     const int kpos0 = pre ? 0 : np;                     // position of key 0
     int lim[MT], qpos[MT], hq[MT];
@@ -274,15 +265,15 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[mt][d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-    auto block = [&](Blk& x) {
+    for (; blk < blk_end; blk += WV) {
         const int j0 = blk * BK;
-        const bool more = blk + PF * WV < blk_end;
+        const bool more = blk + WV < blk_end;
         const bool masked = j0 + BK > nall;
         // ---- scores
-        f32x4_t sc[MT][2 * NB];                         // q . codes; times ksc it is the score in log 2 units
-        float ksc[2 * NB][4];
+        f32x4_t sc[MT][2];                         // q . codes; times ksc it is the score in log 2 units
+        float ksc[2][4];
 #pragma unroll
-        for (int a = 0; a < 2 * NB; ++a) {
+        for (int a = 0; a < 2; ++a) {
             unsigned kf[KF][4];
 #pragma unroll
             for (int q = 0; q < Blk::KC; ++q) {
@@ -333,12 +324,12 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
                 for (int r = 0; r < 4; ++r) ksc[a][r] = 1.f;
         }
-        if (more) ca_load_k<FMT, D, NB>(x, cv, j0 + PF * WV * BK);
+        if (more) ca_load_k<FMT, D>(x, cv, j0 + WV * BK);
         bool odd = false;                               // bf16: a value that is not finite in a block of which some row must not see all
         if (FMT == SMX_KV_BF16 && masked) {
             bool bad = false;
 #pragma unroll
-            for (int a = 0; a < 2 * NB; ++a)
+            for (int a = 0; a < 2; ++a)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -347,7 +338,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             odd = causal && __ballot(bad) != 0;
             if (odd)                                    // (the product leaves them out; the rows that do see them get them below)
 #pragma unroll
-                for (int a = 0; a < 2 * NB; ++a)
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -356,20 +347,20 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                             if ((x.v[a][r][q] & 0x7f800000u) == 0x7f800000u) x.v[a][r][q] &= 0xffffu;
                         }
         }
-        float vsc[2 * NB][4];
+        float vsc[2][4];
 #pragma unroll
-        for (int a = 0; a < 2 * NB; ++a)
+        for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int r = 0; r < 4; ++r) vsc[a][r] = FMT <= SMX_KV_INT8 ? ca_scale(x.vs, a, r) : 1.f;
         // ---- probabilities: one fused product and difference, one exponential.  A probability above 2^16 (also the first ever: the reference
         // starts at the lowest value) sends the row's wave back to the scores for a new reference.
-        unsigned pf[MT][NB][NP][4];
+        unsigned pf[MT][NP][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            f32x4_t pr[2 * NB];
+            f32x4_t pr[2];
             float big = 0.f;
 #pragma unroll
-            for (int a = 0; a < 2 * NB; ++a)
+            for (int a = 0; a < 2; ++a)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     pr[a][r] = ca_exp2(fmaf(sc[mt][a][r], ksc[a][r], -m[mt]));
@@ -378,7 +369,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             if (__ballot(big > CA_BIG)) {
                 float mx = m[mt];
 #pragma unroll
-                for (int a = 0; a < 2 * NB; ++a)
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[mt][a][r] * ksc[a][r]);
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
@@ -389,12 +380,12 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
                 for (int d = 0; d < DT; ++d) acc[mt][d] *= al;
 #pragma unroll
-                for (int a = 0; a < 2 * NB; ++a)
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) pr[a][r] = ca_exp2(fmaf(sc[mt][a][r], ksc[a][r], -mx));
             }
 #pragma unroll
-            for (int a = 0; a < 2 * NB; ++a) {
+            for (int a = 0; a < 2; ++a) {
                 l[mt] += (pr[a][0] + pr[a][1]) + (pr[a][2] + pr[a][3]);
                 if (FMT <= SMX_KV_INT8)
 #pragma unroll
@@ -407,7 +398,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
                     for (int n = 0; n < NP; ++n) {
                         const unsigned h = pack_bf2(pr[a][2 * e], pr[a][2 * e + 1]);
-                        pf[mt][a >> 1][n][2 * (a & 1) + e] = h;
+                        pf[mt][n][2 * a + e] = h;
                         if (n + 1 < NP) {               // what h leaves over: -1 * its half + the number, one instruction
                             pr[a][2 * e] = ca_dot2(h, one_lo, pr[a][2 * e]);
                             pr[a][2 * e + 1] = ca_dot2(h, one_hi, pr[a][2 * e + 1]);
@@ -415,30 +406,26 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                     }
             }
         }
-        // ---- the second product, 32 keys at a time
+        // ---- the second product.  V, register by register of the keys: 4 (bf16: 2) d-tiles of two keys per register
+        enum { DR = 4 / ES };
 #pragma unroll
-        for (int st = 0; st < NB; ++st) {
-            // V, register by register of the keys: 4 (bf16: 2) d-tiles of two keys per register
-            enum { DR = 4 / ES };
+        for (int q = 0; q < Blk::VW; ++q) {
+            unsigned vx[8][DR / 2];
 #pragma unroll
-            for (int q = 0; q < Blk::VW; ++q) {
-                unsigned vx[8][DR / 2];
+            for (int e = 0; e < 8; ++e) {
+                const unsigned u = x.v[e >> 2][e & 3][q];
+                if (ES == 2) vx[e][0] = u;
+                else ca_cvt4<FMT>(u, vx[e][0], vx[e][DR / 2 - 1]);
+            }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const unsigned u = x.v[2 * st + (e >> 2)][e & 3][q];
-                    if (ES == 2) vx[e][0] = u;
-                    else ca_cvt4<FMT>(u, vx[e][0], vx[e][DR / 2 - 1]);
-                }
+            for (int d = 0; d < DR; ++d) {
+                unsigned vf[4];
 #pragma unroll
-                for (int d = 0; d < DR; ++d) {
-                    unsigned vf[4];
+                for (int k = 0; k < 4; ++k) vf[k] = __builtin_amdgcn_perm(vx[2 * k + 1][d >> 1], vx[2 * k][d >> 1], (d & 1) ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) vf[k] = __builtin_amdgcn_perm(vx[2 * k + 1][d >> 1], vx[2 * k][d >> 1], (d & 1) ? 0x07060302u : 0x05040100u);
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int n = NP - 1; n >= 0; --n) acc[mt][DR * q + d] = ca_mfma(vf, pf[mt][st][n], acc[mt][DR * q + d]);
-                }
+                    for (int n = NP - 1; n >= 0; --n) acc[mt][DR * q + d] = ca_mfma(vf, pf[mt][n], acc[mt][DR * q + d]);
             }
         }
         if (FMT == SMX_KV_BF16 && odd) {
@@ -447,7 +434,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                 const bf16_t* v = reinterpret_cast<const bf16_t*>(c.v) + base + (long long)min(j, nmax - 1) * c.ts;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    const unsigned w0 = pf[mt][0][0][0], w1 = pf[mt][0][0][1], w2 = pf[mt][0][0][2], w3 = pf[mt][0][0][3];
+                    const unsigned w0 = pf[mt][0][0], w1 = pf[mt][0][1], w2 = pf[mt][0][2], w3 = pf[mt][0][3];
                     const unsigned u01 = wd & 1 ? w1 : w0, u23 = wd & 1 ? w3 : w2, u = (unsigned)__shfl((int)(wd & 2 ? u23 : u01), src, 64);
                     const float pk = __uint_as_float(k & 1 ? u & 0xffff0000u : u << 16);
                     if (j < lim[mt])
@@ -461,13 +448,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                 }
             }
         }
-        if (more) ca_load_v<FMT, D, NB>(x, cv, j0 + PF * WV * BK);
-        blk += WV;
-    };
-    while (blk < blk_end) {
-#pragma unroll
-        for (int f = 0; f < PF; ++f)
-            if (f == 0 || blk < blk_end) block(buf[f]);
+        if (more) ca_load_v<FMT, D>(x, cv, j0 + WV * BK);
     }
 
     if (WV == 1) {                                      // a wave has all of its rows: out of the registers
@@ -493,7 +474,12 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) Cvt<T>::st(out + DT * (4 * g + q) + d, L == 0.f ? 0.f : acc[mt][d][q] * inv);
+                    for (int d = 0; d < DT; d += 4) {
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = L == 0.f ? 0.f : acc[mt][d + e][q] * inv;
+                        ca_store4(out + DT * (4 * g + q) + d, v);
+                    }
                 if (p.lse && g == 0) p.lse[((long long)bb * p.H + h) * p.Tq + t] = ca_lse(m[mt], L);
             }
         }
@@ -544,7 +530,12 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             const float inv = L == 0.f ? 0.f : 1.f / L;
             T* out = reinterpret_cast<T*>(p.o) + bb * p.o_bs + t * p.o_ts + h * p.o_hs + d0;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) Cvt<T>::st(out + d, L == 0.f ? 0.f : o[d] * inv);
+            for (int d = 0; d < DT; d += 4) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = L == 0.f ? 0.f : o[d + e] * inv;
+                ca_store4(out + d, v);
+            }
             if (p.lse && d0 == 0) p.lse[((long long)bb * p.H + h) * p.Tq + t] = ca_lse(M, L);
         }
     }
@@ -643,7 +634,8 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
         T* out = reinterpret_cast<T*>(p.o) + b * p.o_bs + t * p.o_ts + h * p.o_hs + dl;
         const float inv = 1.f / l;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) Cvt<T>::st(out + d, l == 0.f ? 0.f : o[d] * inv);
+        for (int d = 0; d < 4; ++d) o[d] = l == 0.f ? 0.f : o[d] * inv;
+        ca_store4(out, o);
         if (p.lse && dl == 0) p.lse[id] = ca_lse(m, l);
     }
 }

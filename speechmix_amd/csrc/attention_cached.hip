@@ -115,6 +115,12 @@ static int ca_splits(long long base, int cap, long long want) {
     const long long m = n < most ? n : most;
     return (int)(m < 1 ? 1 : m > 64 ? 64 : m);
 }
+static CaDiv ca_divisor(int d) {
+    CaDiv v = {0u, 0, d};
+    while ((1ll << v.k) < d) ++v.k;
+    v.m = (unsigned)(((1ull << (31 + v.k)) + d - 1) / d);
+    return v;
+}
 static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, CaPlan& pl, long long& items) {
     const SmxKVCache& m = p.own.k ? p.own : p.pre;
     const long long ro = p.own.k ? (long long)p.Tq * pl.G : 0, rp = p.pre.k ? (long long)pl.R * p.Tq * pl.G : 0;
@@ -129,16 +135,12 @@ static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, CaPlan& pl, long lo
     pl.nso = !p.own.k ? 0 : pl.single ? 1 : ca_splits(bo, p.own.cap, want);
     const long long left = want - (pl.single ? 0 : bo * pl.nso);        // (those of short caches are soon gone)
     pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, left > want / 2 ? left : want / 2) : 0;
+    pl.nso_ = ca_divisor(pl.nso > 0 ? pl.nso : 1);
+    pl.nsp_ = ca_divisor(pl.nsp > 0 ? pl.nsp : 1);
     pl.items_p = (int)(bp * pl.nsp);
     pl.items_o = (int)(bo * pl.nso);
     items = bp * pl.nsp + bo * pl.nso;
     pl.join = pl.nso + pl.nsp > 1;
-}
-static CaDiv ca_divisor(int d) {
-    CaDiv v = {0u, 0, d};
-    while ((1ll << v.k) < d) ++v.k;
-    v.m = (unsigned)(((1ull << (31 + v.k)) + d - 1) / d);
-    return v;
 }
 static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long long& items) {
     const SmxKVCache& m = p.own.k ? p.own : p.pre;
@@ -147,6 +149,9 @@ static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long lon
     pl.R = p.pre.k ? p.B / p.pre.B : 1;
     pl.per = ca_divisor(p.Tq * pl.G);
     pl.g = ca_divisor(pl.G);
+    pl.hkv_ = ca_divisor(pl.Hkv);
+    pl.bo_ = ca_divisor(p.own.k ? p.own.B : 1);
+    pl.bp_ = ca_divisor(p.pre.k ? p.pre.B : 1);
     const long long ro = p.own.k ? (long long)p.Tq * pl.G : 0, rp = p.pre.k ? (long long)pl.R * p.Tq * pl.G : 0, rmax = ro > rp ? ro : rp;
     int mt = dtype == SMX_F32 || rmax <= 16 ? 1 : rmax <= 32 || m.D == 128 ? 2 : 4;
     // (own keys that outweigh the prefix's decide: more of their small items are resident beside a small form)

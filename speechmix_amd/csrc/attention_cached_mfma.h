@@ -30,6 +30,7 @@ __device__ __forceinline__ int ca_div(const CaDiv& v, int r) { return (int)(__um
 
 struct CaPlan {
     CaDiv per, g;                 // by Tq * G, by G
+    CaDiv nso_, nsp_, hkv_, bo_, bp_;     // by nso, nsp, Hkv, the entries of either part
     int G, Hkv, R;                // query heads per KV head; rows per prefix
     int mbo, mbp;                 // blocks of 16 * MT rows per (entry, KV head): own, prefix
     int nso, nsp;                 // key splits: own, prefix
@@ -204,7 +205,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
     // keys that the block's first row sees (all rows see them) and that its last row sees
     const int nmax = pre ? np : causal ? max(min(nk, nk - p.Tq + ca_div(pl.g, rlast) + 1), 0) : nk;
     const int nall = causal ? max(nk - p.Tq + ca_div(pl.g, row0) + 1, 0) : nmax;
-    const int nblk = (nmax + BK - 1) / BK, bps = (nblk + ns - 1) / ns;
+    const int nblk = (nmax + BK - 1) / BK, bps = ca_div(pre ? pl.nsp_ : pl.nso_, nblk + ns - 1);
     const int blk_end = min(nblk, (s + 1) * bps);
     const long long base = (long long)b * c.bs + (long long)hk * c.hs, sbase = (long long)b * c.sbs + (long long)hk * c.shs;
     const CaView cv = {(const char*)c.k + base * ES, (const char*)c.v + base * ES, c.ks + sbase, c.vs + sbase, (int)c.ts * ES, nmax,
@@ -387,12 +388,14 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 l[mt] += (pr[a][0] + pr[a][1]) + (pr[a][2] + pr[a][3]);
-                if (FMT <= SMX_KV_INT8)
+                if (FMT <= SMX_KV_INT8) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        pr[a][r] *= vsc[a][r];
-                        if (masked && j0 + 16 * a + 4 * g + r >= lim[mt]) pr[a][r] = 0.f;                  // (its scale may be anything)
-                    }
+                    for (int r = 0; r < 4; ++r) pr[a][r] *= vsc[a][r];
+                    if (masked)                         // (a hidden key's scale may be anything)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (j0 + 16 * a + 4 * g + r >= lim[mt]) pr[a][r] = 0.f;
+                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -562,13 +565,12 @@ __global__ __launch_bounds__(MODE == CA_EIGHT ? 512 : 256, ca_occ(CaFmt<FMT>::ES
     if (single) id = 4 * id + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (single && id >= pl.items_o) return;             // (the last workgroup's spare waves; no barrier in that form)
     it.slot = (it.pre ? 0 : pl.items_p) + (long long)id;
-    const int ns = it.pre ? pl.nsp : pl.nso, cb = it.pre ? p.pre.B : p.own.B;
-    it.s = id % ns;
-    id /= ns;
-    it.hk = id % pl.Hkv;
-    id /= pl.Hkv;
-    it.b = id % cb;
-    it.row0 = id / cb * (16 * MT);
+    const CaDiv &dns = it.pre ? pl.nsp_ : pl.nso_, &dcb = it.pre ? pl.bp_ : pl.bo_;
+    const int q1 = ca_div(dns, id), q2 = ca_div(pl.hkv_, q1), q3 = ca_div(dcb, q2);      // key split fastest, then KV head, entry, block of rows
+    it.s = id - q1 * dns.d;
+    it.hk = q1 - q2 * pl.Hkv;
+    it.b = q2 - q3 * dcb.d;
+    it.row0 = q3 * (16 * MT);
     if (MODE == CA_SINGLE) ca_body<FMT, D, 1, MT, 1, WV, T>(p, pl, it, sh);
     else if (MODE == CA_MIXED && !it.pre) ca_body<FMT, D, 1, MT, 1, WV, T>(p, pl, it, sh);
     else if (MODE == CA_SMALL && !it.pre) ca_body<FMT, D, 1, MT, 4, WV, T>(p, pl, it, sh);

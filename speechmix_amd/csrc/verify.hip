@@ -3,6 +3,8 @@
 //   (q_i is 1 at x_i).  At the first rejected draft r the next token is drawn from max(p_r - q_r, 0); when all n are accepted, or at an id
 //   outside the vocabulary (the end of a shorter draft), from p itself.  Drawing: the smallest index whose running sum exceeds u_n * (the sum of
 //   all weights); sums in 64 bits - the borders of 50 000 intervals lie closer than 32-bit sums are sure of.
+// Bounds: a chain of dependent loads and scans, 5.4 us whatever the size (ids -> probabilities at the ids -> the row -> its sums -> the chosen segment
+// again), and what one CU reads (100 GB/s) of the one or two rows that count: 64 rows of 50 265 with four drafts 11 us, 256 rows without drafts 13 us.
 //   u = null: greedy - draft i is accepted while it equals arg max p_i (ties: the lowest index; target may then hold logits).
 #include "smx_common.h"
 

@@ -1308,9 +1308,9 @@ class KVCache:
     def empty(cls, B, H, cap, D, fmt, device):
         """A cache of zeros (scales of one)."""
         dt = _KV_STORE[fmt][0] if fmt in KV_FORMATS else torch.uint8
-        k = torch.zeros(2, B, H, cap, D, dtype=dt, device=device)
-        s = torch.ones(2, B, H, cap, device=device) if fmt in ("e4m3", "int8") else (None, None)
-        return cls(k[0], k[1], s[0], s[1], fmt)
+        k, v = (torch.zeros(B, H, cap, D, dtype=dt, device=device) for _ in range(2))         # (two allocations: both start aligned)
+        ks, vs = (torch.ones(B, H, cap, device=device) if fmt in ("e4m3", "int8") else None for _ in range(2))
+        return cls(k, v, ks, vs, fmt)
 
     def bytes(self):
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.ks, self.vs) if t is not None)

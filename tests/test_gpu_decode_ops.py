@@ -34,7 +34,7 @@ def _vals(c):
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("B,T,H,D,cap", [(1, 1, 1, 64, 1), (3, 1, 12, 64, 9), (2, 7, 2, 128, 20), (2, 37, 3, 16, 37), (1, 5, 2, 24, 8), (2, 4, 1, 256, 6),
-                                         (1, 130, 2, 8, 200)])
+                                         (1, 130, 2, 8, 200), (1, 3, 1, 40, 3)])
 def test_append_and_read(fmt, dtype, B, T, H, D, cap):
     from speechmix_amd import ops
     g = _gen(B * 1000 + T)
@@ -249,6 +249,52 @@ def test_attention_many_short_rows(fmt, dtype, D, Tq):
     _check(q, c, klen, pre=pre, plen=[20, 0, 7])
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "bf16"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,R_,cap,P", [(64, 49, 0, 70), (64, 64, 0, 33), (128, 21, 0, 70), (64, 18, 0, 40), (64, 49, 260, 3500), (64, 49, 40, 600),
+                                        (128, 21, 260, 5000), (128, 30, 40, 1300), (64, 17, 33, 700)])
+def test_attention_many_rows_of_many_prefixes(fmt, dtype, D, R_, cap, P):
+    """Enough groups that an item takes 32 or 64 rows of a prefix (a few rows are left over), without own keys, with long ones and with short
+    ones: the first, a middle and the last group against the reference."""
+    NG, H = 32, 8
+    B = NG * R_
+    pre = _filled(NG, H, P, D, fmt, 61)
+    q = torch.randn(B, 1, H, D, device="cuda", generator=_gen(62)).to(dtype)
+    plen = [(13 * g) % 70 for g in range(NG - 1)] + [min(P, 70)]
+    c = _filled(B, H, cap, D, fmt, 63) if cap else None
+    klen = [(7 * b) % 38 for b in range(B)] if cap else None
+    rel = torch.randn(H, 50, device="cuda", generator=_gen(64)) if R_ == 49 else None
+    from speechmix_amd import ops
+    kl, pl = (torch.tensor(x, dtype=torch.int32, device="cuda") if x is not None else None for x in (klen, plen))
+    o, lse = ops.attention_cached(q, c, kl, rel_bias=rel, prefix=pre, prefix_len=pl, want_lse=True)
+    for g in (0, 17, NG - 1):
+        rows = slice(g * R_, (g + 1) * R_)
+        vals = []
+        for cc, sl, n in ((c, rows, 38), (pre, slice(g, g + 1), 70)):
+            vals += [R.values(t[sl, :, :n], s[sl, :, :n] if s is not None else None, cc.fmt) for t, s in ((cc.k, cc.ks), (cc.v, cc.vs))] if cc is not None else [None, None]
+        ref = R.attention(q[rows], vals[0], vals[1], klen[rows] if cap else None, [plen[g]], vals[2], vals[3], R_, True, D ** -0.5, rel)
+        tol_o, tol_l = R.attention_bounds(*ref, D, dtype)
+        assert ((o[rows].double().cpu() - ref[0]).abs() <= tol_o).all(), g
+        empty = torch.isinf(ref[1])
+        assert torch.equal(torch.isinf(lse[rows].cpu()), empty) and ((lse[rows].double().cpu() - ref[1]).abs()[~empty] <= tol_l[~empty]).all(), g
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
+def test_attention_many_queries_of_many_rows(fmt):
+    """64 and more rows a KV head out of queries and grouped heads, causal, in items of several tiles."""
+    B, Tq, Hkv, G = 40, 33, 8, 2
+    c = _filled(B, Hkv, 70, 64, fmt, 65)
+    q = torch.randn(B, Tq, Hkv * G, 64, device="cuda", generator=_gen(66)).to(torch.bfloat16)
+    klen = [(9 * b) % 71 for b in range(B)]
+    from speechmix_amd import ops
+    o, _ = ops.attention_cached(q, c, torch.tensor(klen, dtype=torch.int32, device="cuda"))
+    for b in (0, 7, 39):
+        ref = R.attention(q[b:b + 1], *(R.values(t[b:b + 1], s[b:b + 1] if s is not None else None, fmt) for t, s in ((c.k, c.ks), (c.v, c.vs))), klen[b:b + 1], None,
+                          None, None, 1, True, 64 ** -0.5, None)
+        tol_o, _ = R.attention_bounds(*ref, 64, q.dtype)
+        assert ((o[b:b + 1].double().cpu() - ref[0]).abs() <= tol_o).all(), b
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_long_cache_is_split_and_joined(fmt, dtype):
@@ -291,6 +337,24 @@ def test_what_lies_behind_the_last_token_never_counts(fmt, D):
     got, gl = ops.attention_cached(q, c, klen, want_lse=True)
     assert torch.equal(want[:, :2], got[:, :2]) and torch.equal(wl[..., :2], gl[..., :2])
     assert torch.isnan(got[0, 2]).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_hidden_tokens_in_items_of_several_tiles(fmt, D):
+    """What causality hides from a query may hold NaN and infinities, also where a wave has 32 or 64 rows."""
+    from speechmix_amd import ops
+    B, Tq, H, cap = 80, 40, 8, 64
+    c = _filled(B, H, cap, D, fmt, 67)
+    q = torch.randn(B, Tq, H, D, device="cuda", generator=_gen(68)).to(torch.bfloat16)
+    klen = torch.full((B,), 60, dtype=torch.int32, device="cuda")
+    want, _ = ops.attention_cached(q, c, klen)
+    bad = torch.full((B, 1, H, D), float("nan"), device="cuda")
+    bad[::2] = float("inf")
+    ops.kv_append(c, bad, bad, klen - 3)
+    got, _ = ops.attention_cached(q, c, klen)
+    assert torch.equal(want[:, :Tq - 3], got[:, :Tq - 3])
+    assert not torch.isfinite(got[:, Tq - 3:]).any()
 
 
 def test_attention_over_the_decoder_own_interleaved_cache():

@@ -100,7 +100,7 @@ class CachedDecoder:
         if not g:                                       # (False: capture was refused, this width stays eager)
             self.warm.add(Tq)
             return self._step(ids)
-        graph, buf, logits = g
+        graph, buf, logits, _ = g
         buf.copy_(ids)
         graph.replay()
         return logits
@@ -118,7 +118,8 @@ class CachedDecoder:
         finally:
             if gc_was:
                 gc.enable()
-        return graph, buf, logits
+        # (the graph holds addresses: a workspace of the engine that a wider step replaces must outlive it)
+        return graph, buf, logits, self.eng.workspaces()
 
     def _step(self, ids):
         eng, lc = self.eng, self.eng.lc

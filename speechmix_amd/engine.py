@@ -445,6 +445,11 @@ class Engine:
             self._persist[key] = t
         return t
 
+    def workspaces(self):
+        """The scratch tensors of this moment.  Whoever captures launches that may use them keeps the list: a buffer that grows is replaced,
+        and a graph must not write where the allocator has put something else since."""
+        return [t for t in self._persist.values() if isinstance(t, torch.Tensor)]
+
     def W(self, n): return self.st.w(n)
     def P(self, n): return self.st.p32(n)
     def G(self, n): return self.st.g(n)

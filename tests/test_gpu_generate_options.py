@@ -190,6 +190,29 @@ def test_replayed_steps_equal_eager_ones(lm, monkeypatch):
     assert rows[0] == rows[1]
 
 
+def test_a_replayed_step_leaves_replaced_workspaces_alone():
+    """A feed-forward that splits its reduction takes a scratch buffer of the engine, and a wider step replaces that buffer: the narrow step's
+    graph still runs on the old one, which nothing else may be given meanwhile."""
+    from speechmix_amd.decoding import CachedDecoder
+    model = _model(dict(BART, decoder_ffn_dim=2048), "bf16")
+    eng = model.engine
+    with torch.no_grad():
+        enc, B, S = model._speech_encode(_wave(2))
+        eng._persist.pop("fwd_slabs", None)
+        dec = CachedDecoder(eng, enc, B, S, 2, 40, "fp8")
+        ids = torch.full((4, 1), 7, dtype=torch.int64, device=model.device)
+        want = [dec.step(ids).clone() for _ in range(3)][-1]
+        old = eng._persist["fwd_slabs"]
+        size, where = old.numel(), old.data_ptr()
+        del old
+        dec.step(ids.expand(4, 24).contiguous())
+        assert eng._persist["fwd_slabs"].data_ptr() != where
+        canaries = [torch.full((size,), 3.0, device=model.device) for _ in range(16)]
+        got = dec.step(ids).clone()
+        assert torch.equal(got, want) and all((c == 3.0).all() for c in canaries)
+        assert all(c.data_ptr() != where for c in canaries)
+
+
 @pytest.mark.parametrize("kv", [None, "fp8"])
 def test_sampled_rows(kv):
     """Rows per clip, seeds, temperatures."""

@@ -1978,7 +1978,7 @@ class Engine:
                        nxt=torch.empty(B, dtype=torch.int64, device=self.dev), done=torch.zeros(B, dtype=torch.bool, device=self.dev),
                        out=torch.empty(B, Lmax, dtype=torch.int64, device=self.dev), lse=self.new(B * H, dt=torch.float32),
                        pbias=torch.empty(H, Lmax, Lmax, dtype=torch.float32, device=self.dev) if t5 else None,
-                       fin=torch.empty((), dtype=torch.int64, device=self.dev), graphs={}, calls=0, pool=None, eager_done=set(),
+                       fin=torch.empty((), dtype=torch.int64, device=self.dev), graphs={}, keep={}, calls=0, pool=None, eager_done=set(),
                        failures=0)
             stt["bytes"] = sum(t.numel() * t.element_size() for t in stt["xkv"] + stt["cache"] + [stt["logits"]])
             if use_graphs:
@@ -2105,6 +2105,7 @@ class Engine:
                     if stt["pool"] is None:
                         stt["pool"] = g.pool()
                     stt["graphs"][t] = g
+                    stt["keep"].update((w.data_ptr(), w) for w in self.workspaces())       # (see there)
                 g.replay()
             else:
                 step(t)

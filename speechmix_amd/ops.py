@@ -1426,7 +1426,7 @@ def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel
     new ones included; None: the whole capacity) behind an optional `prefix` cache: entry g of it is shared by the B / prefix.B consecutive
     rows of group g (prefix_len int32 [groups]) and seen by all their queries.  cache = None: only the prefix.  `causal` orders the new
     tokens among themselves.  H may be a multiple of the caches' heads.  scale: D ** -0.5 unless given.  rel_bias fp32 [H, n]: bias by the
-    distance query - key, clamped to 0 .. n - 1.  A query that sees no key gives zeros and lse = -inf.
+    distance query - key, clamped to 0 .. n - 1.  A query that sees no key gives zeros and lse = -inf.  An inference operator: it has no backward.
     -> (out [B, Tq, H, D] of q's type, lse fp32 [B, H, Tq] or None)."""
     causal, scale = bool(causal), None if scale is None else float(scale)          # (values, not objects, in the signature)
     sig = (_sig(q), cache.signature if cache is not None else None, prefix.signature if prefix is not None else None, torch._C._cuda_getDevice(),

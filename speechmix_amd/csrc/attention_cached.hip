@@ -121,7 +121,7 @@ static CaDiv ca_divisor(int d) {
     v.m = (unsigned)(((1ull << (31 + v.k)) + d - 1) / d);
     return v;
 }
-static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, CaPlan& pl, long long& items) {
+static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, bool all1, CaPlan& pl, long long& items) {
     const SmxKVCache& m = p.own.k ? p.own : p.pre;
     const long long ro = p.own.k ? (long long)p.Tq * pl.G : 0, rp = p.pre.k ? (long long)pl.R * p.Tq * pl.G : 0;
     pl.mbo = ca_cdiv(ro, 16 * mt);
@@ -131,10 +131,10 @@ static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, CaPlan& pl, long lo
     const long long want = mt == 1 && m.D == 64 ? 1024 : 512;
     // a wave per item where there are many items of few keys: a workgroup's other three waves would have nothing to do (16 384 rows and heads of
     // 43 keys behind prefixes: 151 us with a workgroup each, 55 so)
-    pl.single = p.own.k && ro <= 16 && p.own.cap <= CA_SHORT && bo > 512;
+    pl.single = all1 ? 2 : p.own.k && ro <= 16 && p.own.cap <= CA_SHORT && bo > 512;
     pl.nso = !p.own.k ? 0 : pl.single ? 1 : ca_splits(bo, p.own.cap, want);
     const long long left = want - (pl.single ? 0 : bo * pl.nso);        // (those of short caches are soon gone)
-    pl.nsp = p.pre.k ? ca_splits(bp, p.pre.cap, left > want / 2 ? left : want / 2) : 0;
+    pl.nsp = !p.pre.k ? 0 : all1 ? 1 : ca_splits(bp, p.pre.cap, left > want / 2 ? left : want / 2);
     pl.nso_ = ca_divisor(pl.nso > 0 ? pl.nso : 1);
     pl.nsp_ = ca_divisor(pl.nsp > 0 ? pl.nsp : 1);
     pl.items_p = (int)(bp * pl.nsp);
@@ -147,6 +147,7 @@ static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long lon
     pl.Hkv = m.H;
     pl.G = p.H / m.H;
     pl.R = p.pre.k ? p.B / p.pre.B : 1;
+    pl.r_ = ca_divisor(pl.R);
     pl.per = ca_divisor(p.Tq * pl.G);
     pl.g = ca_divisor(pl.G);
     pl.hkv_ = ca_divisor(pl.Hkv);
@@ -156,12 +157,23 @@ static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long lon
     int mt = dtype == SMX_F32 || rmax <= 16 ? 1 : rmax <= 32 || m.D == 128 ? 2 : 4;
     // (own keys that outweigh the prefix's decide: more of their small items are resident beside a small form)
     if (p.own.k && p.pre.k && ro <= 16 && (long long)p.own.B * p.own.cap > (rp + 15) / 16 * p.pre.B * (long long)p.pre.cap) mt = 1;
-    ca_plan_mt(p, mt, pl, items);
+    // Every item to a wave of its own, 16 rows each: a prefix's keys are converted again for every 16 of its rows, but no waves have to meet.  With
+    // own keys where those are many and short and the prefix is not long (16 384 rows and heads of 17 keys behind 16 prefixes of 450, D 64: 39.2 us
+    // in items of 64 rows, 29.6 so; of 100: 27.1 and 25.1; 4 096 of them: no gain); a prefix alone where the rows are many, but not the keys, of
+    // bf16 of 64 or fp32 of 128 (16 prefixes x 16 heads x 64 rows, bf16, D 64, 60 keys: 9.3 and 7.0, 250: 11.3 and 10.4, 500: 15.0 and 19.8; fp32,
+    // D 128, 30 keys: 14.1 and 9.6, 250: 20.4 and 19.3; against it bf16, D 128, 200 keys: 11.9 and 14.5, and fp32, D 64, 60 keys: 7.8 and 8.3).
+    const bool all1 = p.own.k && p.pre.k ? ro <= 16 && (long long)p.own.B * pl.Hkv >= 8192 && p.own.cap <= CA_SHORT && p.pre.cap <= 2 * CA_SHORT
+                    : p.pre.k && rp > 16 && (rp + 15) / 16 * p.pre.B * pl.Hkv >= 1024 && p.pre.cap <= CA_SHORT && (m.D == 64) == (dtype == SMX_BF16);
+    if (all1) {
+        ca_plan_mt(p, 1, true, pl, items);
+        return 1;
+    }
+    ca_plan_mt(p, mt, false, pl, items);
     // Fewer rows per item while that leaves CUs idle: a block of keys takes 2.5 us for 64 rows and 0.9 for 16 (33 rows x 171 keys x 12 heads: 11.0 us
     // in 12 workgroups, 5.7 in 36).
     while (mt > 1 && items < 256) {
         mt >>= 1;
-        ca_plan_mt(p, mt, pl, items);
+        ca_plan_mt(p, mt, false, pl, items);
     }
     return mt;
 }
@@ -211,7 +223,8 @@ extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp
 
 #define CA_JOIN_T(D, T)                                                                                                               \
     do {                                                                                                                              \
-        if (wide) hipLaunchKernelGGL((attn_cached_join<D, 4, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                          \
+        if (pair) hipLaunchKernelGGL((attn_cached_join2<D, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                            \
+        else if (wide) hipLaunchKernelGGL((attn_cached_join<D, 4, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                          \
         else hipLaunchKernelGGL((attn_cached_join<D, 1, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                               \
     } while (0)
 #define CA_JOIN(D)                                 \
@@ -230,7 +243,7 @@ extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hi
         CaPlan pl;
         long long items;
         const int mt = ca_plan(p, dtype, pl, items);
-        if (items > 0x7fffffffll) return SMX_EINVAL;
+        if (items > 0x7fffffffll || (pl.join && (long long)p.B * p.H * p.Tq > 0x7fffffffll)) return SMX_EINVAL;
         if (pl.join) {
             const long long rows = items * 16 * mt;
             if (!p.ws || ((size_t)p.ws & 15) || p.ws_bytes < rows * (D + 2) * 4) return SMX_EINVAL;
@@ -241,8 +254,8 @@ extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hi
         // keys a workgroup may have to go through; eight waves halve that where the chip has room for them (32 x 16 heads x 777 keys, five queries:
         // 13.5 -> 12.2 us; heads of 128 have no room: 64 x 8 x 512 11.6 -> 14.3)
         const int keys = std::max(p.own.k ? p.own.cap / pl.nso : 0, p.pre.k ? p.pre.cap / pl.nsp : 0);
-        const int mode = pl.single ? (p.pre.k ? CA_MIXED : CA_SINGLE) : mt > 1 && few ? CA_SMALL : mt == 1 && D == 64 && items <= 512 && keys >= 256 ? CA_EIGHT : CA_PLAIN;
-        const dim3 grid((unsigned)(pl.items_p + (pl.single ? (pl.items_o + 3) / 4 : pl.items_o)));
+        const int mode = pl.single ? (p.pre.k && pl.single == 1 ? CA_MIXED : CA_SINGLE) : mt > 1 && few ? CA_SMALL : mt == 1 && D == 64 && items <= 512 && keys >= 256 ? CA_EIGHT : CA_PLAIN;
+        const dim3 grid((unsigned)(mode == CA_SINGLE ? (items + 3) / 4 : pl.items_p + (pl.single ? (pl.items_o + 3) / 4 : pl.items_o)));
         if (fmt == SMX_KV_E4M3) CA_MFMA(SMX_KV_E4M3);
         else if (fmt == SMX_KV_INT8) CA_MFMA(SMX_KV_INT8);
         else CA_MFMA(SMX_KV_BF16);
@@ -250,7 +263,10 @@ extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hi
             const long long rows = (long long)p.B * p.H * p.Tq;
             // a workgroup per row where there are many splits to add (64 splits of 128 wide: 7.7 us by a wave, 5.3 by four)
             const bool wide = pl.nso > 8 || pl.nsp > 8;
-            const dim3 jg((unsigned)(wide ? rows : (rows + 3) / 4));
+            // (16 384 rows, D 64, of one split each: 17.0 us with a wave per row, 5.0 so)
+            const bool pair = pl.nso == 1 && pl.nsp == 1;
+            const int per = pair ? 1024 / D : wide ? 1 : 4;
+            const dim3 jg((unsigned)((rows + per - 1) / per));
             if (D == 64) CA_JOIN(64);
             else CA_JOIN(128);
         }

@@ -35,13 +35,13 @@ __device__ __forceinline__ int ca_div(const CaDiv& v, int r) { return (int)(__um
 
 struct CaPlan {
     CaDiv per, g;                 // by Tq * G, by G
-    CaDiv nso_, nsp_, hkv_, bo_, bp_;     // by nso, nsp, Hkv, the entries of either part
+    CaDiv nso_, nsp_, hkv_, bo_, bp_, r_; // by nso, nsp, Hkv, the entries of either part, R
     int G, Hkv, R;                // query heads per KV head; rows per prefix
     int mbo, mbp;                 // blocks of 16 * MT rows per (entry, KV head): own, prefix
     int nso, nsp;                 // key splits: own, prefix
     int items_p;                  // work items = workgroups of the prefix part (they come first)
     int items_o;                  // work items of the own part
-    int single;                   // own part: a wave per item, four items per workgroup (short caches, many rows)
+    int single;                   // a wave per item, four items per workgroup (short caches, many rows): 1 own items, 2 all items
     int join;                     // partial results to po / pml instead of the output
     float *po, *pml;              // [item][16 MT][D], [item][16 MT][2]
 };
@@ -554,7 +554,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
 // instructions lie between those that run), as much as a short cache takes.
 enum {
     CA_PLAIN = 0,       // every item: 16 * MT rows by four waves
-    CA_SINGLE = 1,      // own keys only, an item per wave
+    CA_SINGLE = 1,      // a wave per item of 16 rows, four items per workgroup
     CA_SMALL = 2,       // prefix items as in CA_PLAIN, own items of up to 16 rows by four waves
     CA_MIXED = 3,       // prefix items as in CA_PLAIN, own items by a wave each
     CA_EIGHT = 4        // CA_PLAIN with eight waves
@@ -564,11 +564,13 @@ __global__ __launch_bounds__(MODE == CA_EIGHT ? 512 : 256, ca_occ(CaFmt<FMT>::ES
     enum { WV = MODE == CA_EIGHT ? 8 : 4 };
     __shared__ CaShared<D, WV> sh;
     CaItem it;
-    it.pre = MODE != CA_SINGLE && blockIdx.x < (unsigned)pl.items_p;
-    const bool single = MODE == CA_SINGLE || (MODE == CA_MIXED && !it.pre);
-    int id = it.pre ? blockIdx.x : blockIdx.x - pl.items_p;
-    if (single) id = 4 * id + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (single && id >= pl.items_o) return;             // (the last workgroup's spare waves; no barrier in that form)
+    int id = blockIdx.x;
+    if (MODE == CA_SINGLE) id = 4 * id + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (MODE == CA_SINGLE && id >= pl.items_p + pl.items_o) return;      // (the last workgroup's spare waves; no barrier in that form)
+    it.pre = id < pl.items_p;
+    if (!it.pre) id -= pl.items_p;
+    if (MODE == CA_MIXED && !it.pre) id = 4 * id + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (MODE == CA_MIXED && !it.pre && id >= pl.items_o) return;
     it.slot = (it.pre ? 0 : pl.items_p) + (long long)id;
     const CaDiv &dns = it.pre ? pl.nsp_ : pl.nso_, &dcb = it.pre ? pl.bp_ : pl.bo_;
     const int q1 = ca_div(dns, id), q2 = ca_div(pl.hkv_, q1), q3 = ca_div(dcb, q2);      // key split fastest, then KV head, entry, block of rows
@@ -582,23 +584,46 @@ __global__ __launch_bounds__(MODE == CA_EIGHT ? 512 : 256, ca_occ(CaFmt<FMT>::ES
     else ca_body<FMT, D, MT, MT, WV, WV, T>(p, pl, it, sh);
 }
 
+// The id-th of a join's rows: ids go by (entry, KV head, query, head of the group), the order of the partial rows.
+struct CaJoinRow { int b, hk, h, t, r, e, rp; };        // r of its entry's rows; entry e of the prefix and the row of those
+__device__ __forceinline__ CaJoinRow ca_join_row(const SmxCachedAttnParams& p, const CaPlan& pl, int id) {
+    CaJoinRow w;
+    const int u = ca_div(pl.per, id);
+    w.r = id - u * pl.per.d;
+    w.b = ca_div(pl.hkv_, u);
+    w.hk = u - w.b * pl.Hkv;
+    w.t = ca_div(pl.g, w.r);
+    w.h = w.hk * pl.G + w.r - w.t * pl.G;
+    w.e = ca_div(pl.r_, w.b);
+    w.rp = (w.b - w.e * pl.R) * pl.per.d + w.r;
+    return w;
+}
+template <int D, typename T>
+__device__ __forceinline__ void ca_join_store(const SmxCachedAttnParams& p, const CaJoinRow& w, int dl, float m, float l, float o[4]) {
+    T* out = reinterpret_cast<T*>(p.o) + w.b * p.o_bs + w.t * p.o_ts + w.h * p.o_hs + dl;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = l == 0.f ? 0.f : o[d] * inv;
+    ca_store4(out, o);
+    if (p.lse && dl == 0) p.lse[((long long)w.b * p.H + w.h) * p.Tq + w.t] = ca_lse(m, l);
+}
+
 // O = sum over the splits of both parts, in a fixed order: JW waves per (row, head, query), D / 4 lanes per split.  A lane's loads depend on nothing but
 // the weights, and with four waves even 64 splits are four (D = 128: eight) of them.
 template <int D, int JW, typename T>
 __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, CaPlan pl, int mt16) {
     enum { LD = D / 4, NG = 64 / LD * JW };
     const int lane = threadIdx.x & 63, tid = JW == 4 ? threadIdx.x : lane;
-    const long long id = JW == 4 ? (long long)blockIdx.x : (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= (long long)p.B * p.H * p.Tq) return;
-    const int t = (int)(id % p.Tq), h = (int)(id / p.Tq % p.H), b = (int)(id / ((long long)p.Tq * p.H)), hk = h / pl.G;
+    const int id = JW == 4 ? blockIdx.x : blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (id >= p.B * p.H * p.Tq) return;
+    const CaJoinRow w = ca_join_row(p, pl, id);
     const int grp = tid / LD, dl = tid % LD * 4;
     float m = CA_LOWEST, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int part = 0; part < 2; ++part) {
         const SmxKVCache& c = part ? p.own : p.pre;
         if (!c.k) continue;
-        const int ns = part ? pl.nso : pl.nsp, e = part ? b : b / pl.R;
-        const int r = (part ? 0 : b % pl.R * p.Tq * pl.G) + t * pl.G + h % pl.G;
-        const long long it = (part ? pl.items_p : 0) + (((long long)(r / mt16) * c.B + e) * pl.Hkv + hk) * ns;
+        const int ns = part ? pl.nso : pl.nsp, e = part ? w.b : w.e, r = part ? w.r : w.rp;
+        const long long it = (part ? pl.items_p : 0) + (((long long)(r / mt16) * c.B + e) * pl.Hkv + w.hk) * ns;
         const float* po = pl.po + (it * mt16 + r % mt16) * D + dl;
         const long long step = (long long)mt16 * D;
         // at most 64 splits: a lane holds one's maximum and sum
@@ -640,12 +665,22 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] = (so[0][dl + d] + so[1][dl + d]) + (so[2][dl + d] + so[3][dl + d]);
     }
-    if (grp == 0) {
-        T* out = reinterpret_cast<T*>(p.o) + b * p.o_bs + t * p.o_ts + h * p.o_hs + dl;
-        const float inv = 1.f / l;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) o[d] = l == 0.f ? 0.f : o[d] * inv;
-        ca_store4(out, o);
-        if (p.lse && dl == 0) p.lse[id] = ca_lse(m, l);
-    }
+    if (grp == 0) ca_join_store<D, T>(p, w, dl, m, l, o);
+}
+
+// The same where each part has one split (prefixes and own keys that are both short): D / 4 lanes per row and nothing to pass between them.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void attn_cached_join2(SmxCachedAttnParams p, CaPlan pl, int mt16) {
+    enum { LD = D / 4 };
+    const int id = blockIdx.x * (256 / LD) + threadIdx.x / LD, dl = threadIdx.x % LD * 4;
+    if (id >= p.B * p.H * p.Tq) return;
+    const CaJoinRow w = ca_join_row(p, pl, id);
+    const long long ia = (((long long)(w.rp / mt16) * p.pre.B + w.e) * pl.Hkv + w.hk) * mt16 + w.rp % mt16;
+    const long long ib = (pl.items_p + ((long long)(w.r / mt16) * p.own.B + w.b) * pl.Hkv + w.hk) * mt16 + w.r % mt16;
+    const float2 qa = *reinterpret_cast<const float2*>(pl.pml + 2 * ia), qb = *reinterpret_cast<const float2*>(pl.pml + 2 * ib);
+    const float4 a = *reinterpret_cast<const float4*>(pl.po + ia * D + dl), c = *reinterpret_cast<const float4*>(pl.po + ib * D + dl);
+    const float m = fmaxf(qa.x, qb.x);
+    const float fa = qa.y == 0.f ? 0.f : ca_exp2(qa.x - m), fb = qb.y == 0.f ? 0.f : ca_exp2(qb.x - m);
+    float o[4] = {fmaf(c.x, fb, a.x * fa), fmaf(c.y, fb, a.y * fa), fmaf(c.z, fb, a.z * fa), fmaf(c.w, fb, a.w * fa)};
+    ca_join_store<D, T>(p, w, dl, m, fmaf(qb.y, fb, qa.y * fa), o);
 }

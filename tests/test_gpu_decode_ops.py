@@ -279,6 +279,35 @@ def test_attention_many_rows_of_many_prefixes(fmt, dtype, D, R_, cap, P):
         assert torch.equal(torch.isinf(lse[rows].cpu()), empty) and ((lse[rows].double().cpu() - ref[1]).abs()[~empty] <= tol_l[~empty]).all(), g
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "bf16"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,NG,R_,Hkv,G,Tq,cap,P", [(64, 43, 24, 8, 1, 1, 20, 300), (128, 43, 24, 8, 2, 2, 20, 300), (64, 9, 115, 8, 1, 3, 33, 40), (64, 17, 61, 16, 1, 1, 0, 90),
+                                                    (128, 17, 61, 16, 1, 1, 0, 90), (64, 17, 21, 16, 2, 2, 0, 250)])
+def test_attention_an_item_per_wave(fmt, dtype, D, NG, R_, Hkv, G, Tq, cap, P):
+    """So many rows that every wave works for itself, prefixes included, and a row has one partial result of each part: groups without a prefix,
+    rows without a key of their own, rows with neither."""
+    from speechmix_amd import ops
+    B, H = NG * R_, Hkv * G
+    pre = _filled(NG, Hkv, P, D, fmt, 71)
+    q = torch.randn(B, Tq, H, D, device="cuda", generator=_gen(72)).to(dtype)
+    plen = [P] + [(29 * g) % (P + 1) for g in range(1, NG - 1)] + [0]
+    c = _filled(B, Hkv, cap, D, fmt, 73) if cap else None
+    klen = [(7 * b) % (cap + 1) for b in range(B)] if cap else None
+    rel = torch.randn(H, 9, device="cuda", generator=_gen(74)) if G == 2 else None
+    kl, pl = (torch.tensor(x, dtype=torch.int32, device="cuda") if x is not None else None for x in (klen, plen))
+    o, lse = ops.attention_cached(q, c, kl, rel_bias=rel, prefix=pre, prefix_len=pl, want_lse=True)
+    for g in (0, NG // 2, NG - 1):
+        rows = slice(g * R_, (g + 1) * R_)
+        vals = []
+        for cc, sl in ((c, rows), (pre, slice(g, g + 1))):
+            vals += [R.values(t[sl], s[sl] if s is not None else None, cc.fmt) for t, s in ((cc.k, cc.ks), (cc.v, cc.vs))] if cc is not None else [None, None]
+        ref = R.attention(q[rows], vals[0], vals[1], klen[rows] if cap else None, [plen[g]], vals[2], vals[3], R_, True, D ** -0.5, rel)
+        tol_o, tol_l = R.attention_bounds(*ref, D, dtype)
+        assert ((o[rows].double().cpu() - ref[0]).abs() <= tol_o).all(), g
+        empty = torch.isinf(ref[1])
+        assert torch.equal(torch.isinf(lse[rows].cpu()), empty) and ((lse[rows].double().cpu() - ref[1]).abs()[~empty] <= tol_l[~empty]).all(), g
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
 def test_attention_many_queries_of_many_rows(fmt):
     """64 and more rows a KV head out of queries and grouped heads, causal, in items of several tiles."""

@@ -83,7 +83,7 @@ static int ca_check(const SmxCachedAttnParams& p, int dtype) {
     if (p.H % (p.own.k ? p.own.H : p.pre.H)) return SMX_EINVAL;
     if (p.rel_bias && p.nrel <= 0) return SMX_EINVAL;
     if ((((size_t)p.q | (size_t)p.o) & 15) || ((p.q_bs | p.q_ts | p.q_hs | p.o_bs | p.o_ts | p.o_hs) & 7)) return SMX_EINVAL;
-    if ((long long)p.B * p.H * p.Tq > 0x7fffffffll) return SMX_EINVAL;
+    if ((long long)p.B * p.H * p.Tq > 0x7fff0000ll) return SMX_EINVAL;
     // positions and key counts are 32-bit
     if ((long long)(p.own.k ? p.own.cap : 0) + (p.pre.k ? p.pre.cap : 0) + p.Tq > 0x7fff0000ll) return SMX_EINVAL;
     return SMX_OK;
@@ -141,6 +141,9 @@ static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, bool all1, CaPlan& 
     pl.items_o = (int)(bo * pl.nso);
     items = bp * pl.nsp + bo * pl.nso;
     pl.join = pl.nso + pl.nsp > 1;
+    pl.mtl = mt == 1 ? 4 : mt == 2 ? 5 : 6;
+    pl.so = pl.mbo == 1 ? (int)ro : 16 * mt;
+    pl.sp = pl.mbp == 1 ? (int)rp : 16 * mt;
 }
 static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long long& items) {
     const SmxKVCache& m = p.own.k ? p.own : p.pre;
@@ -178,14 +181,16 @@ static int ca_plan(const SmxCachedAttnParams& p, int dtype, CaPlan& pl, long lon
     return mt;
 }
 
+static long long ca_prows(const CaPlan& pl) { return (long long)pl.items_p * pl.sp + (long long)pl.items_o * pl.so; }
+
 // bytes of workspace smx_attention_cached needs for these sizes (0: none)
 extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp, int dtype) {
     if (ca_check(*pp, dtype)) return SMX_EINVAL;
     if (!ca_mfma_ok(*pp)) return 0;
     CaPlan pl;
     long long items;
-    const int mt = ca_plan(*pp, dtype, pl, items);
-    return pl.join ? items * 16 * mt * ((pp->own.k ? pp->own.D : pp->pre.D) + 2) * 4 : 0;
+    ca_plan(*pp, dtype, pl, items);
+    return pl.join ? ca_prows(pl) * ((pp->own.k ? pp->own.D : pp->pre.D) + 2) * 4 : 0;
 }
 
 #define CA_SIMPLE(FMT)                                                                                                                \
@@ -223,9 +228,9 @@ extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp
 
 #define CA_JOIN_T(D, T)                                                                                                               \
     do {                                                                                                                              \
-        if (pair) hipLaunchKernelGGL((attn_cached_join2<D, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                            \
-        else if (wide) hipLaunchKernelGGL((attn_cached_join<D, 4, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                          \
-        else hipLaunchKernelGGL((attn_cached_join<D, 1, T>), jg, dim3(256), 0, stream, p, pl, 16 * mt);                               \
+        if (pair) hipLaunchKernelGGL((attn_cached_join2<D, T>), jg, dim3(256), 0, stream, p, pl);                            \
+        else if (wide) hipLaunchKernelGGL((attn_cached_join<D, 4, T>), jg, dim3(256), 0, stream, p, pl);                          \
+        else hipLaunchKernelGGL((attn_cached_join<D, 1, T>), jg, dim3(256), 0, stream, p, pl);                               \
     } while (0)
 #define CA_JOIN(D)                                 \
     do {                                           \
@@ -243,9 +248,9 @@ extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hi
         CaPlan pl;
         long long items;
         const int mt = ca_plan(p, dtype, pl, items);
-        if (items > 0x7fffffffll || (pl.join && (long long)p.B * p.H * p.Tq > 0x7fffffffll)) return SMX_EINVAL;
+        if (items > 0x7fffffffll) return SMX_EINVAL;
         if (pl.join) {
-            const long long rows = items * 16 * mt;
+            const long long rows = ca_prows(pl);
             if (!p.ws || ((size_t)p.ws & 15) || p.ws_bytes < rows * (D + 2) * 4) return SMX_EINVAL;
             pl.po = (float*)p.ws;
             pl.pml = pl.po + rows * D;

@@ -43,7 +43,8 @@ struct CaPlan {
     int items_o;                  // work items of the own part
     int single;                   // a wave per item, four items per workgroup (short caches, many rows): 1 own items, 2 all items
     int join;                     // partial results to po / pml instead of the output
-    float *po, *pml;              // [item][16 MT][D], [item][16 MT][2]
+    int sp, so, mtl;              // partial rows of an item of either part: 2^mtl = 16 MT, or all its rows where those are fewer
+    float *po, *pml;              // [partial row][D], [partial row][2]: the prefix's items, then the others
 };
 
 template <int FMT> struct CaFmt;
@@ -187,7 +188,7 @@ template <int D, int WV> struct CaShared {       // where the waves meet
     float m[WV][16], l[WV][16];
     __attribute__((aligned(16))) float o[WV][16][D + 4];
 };
-struct CaItem { bool pre; int s, hk, b, row0; long long slot; };      // key split, KV head, batch entry, first row; number among all items
+struct CaItem { bool pre; int s, hk, b, row0; long long prow; };      // key split, KV head, batch entry, first row; first partial row
 
 // One work item: 16 * MT rows (as many as there are of the kernel's 16 * MTB) over one split of the keys, by the workgroup's WV = 4 or 8 waves or by one
 template <int FMT, int D, int MT, int MTB, int WV, int SW, typename T>
@@ -468,7 +469,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             const int r = row0 + 16 * mt + i;
             if (r >= nrows) continue;
             if (pl.join) {
-                const long long pr = it.slot * (16 * MTB) + 16 * mt + i;
+                const long long pr = it.prow + 16 * mt + i;
                 if (g == 0) *reinterpret_cast<float2*>(pl.pml + 2 * pr) = make_float2(m[mt], L);
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
@@ -525,7 +526,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             for (int d = 0; d < DT; ++d) o[d] = fmaf(sh.o[v][row][d0 + d], f, o[d]);
         }
         if (pl.join) {
-            const long long pr = it.slot * (16 * MTB) + 16 * mt + row;
+            const long long pr = it.prow + 16 * mt + row;
             if (r < nrows) {
                 if (d0 == 0) {
                     pl.pml[2 * pr] = M;
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(MODE == CA_EIGHT ? 512 : 256, ca_occ(CaFmt<FMT>::ES
     if (!it.pre) id -= pl.items_p;
     if (MODE == CA_MIXED && !it.pre) id = 4 * id + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (MODE == CA_MIXED && !it.pre && id >= pl.items_o) return;
-    it.slot = (it.pre ? 0 : pl.items_p) + (long long)id;
+    it.prow = it.pre ? (long long)id * pl.sp : (long long)pl.items_p * pl.sp + (long long)id * pl.so;
     const CaDiv &dns = it.pre ? pl.nsp_ : pl.nso_, &dcb = it.pre ? pl.bp_ : pl.bo_;
     const int q1 = ca_div(dns, id), q2 = ca_div(pl.hkv_, q1), q3 = ca_div(dcb, q2);      // key split fastest, then KV head, entry, block of rows
     it.s = id - q1 * dns.d;
@@ -598,6 +599,12 @@ __device__ __forceinline__ CaJoinRow ca_join_row(const SmxCachedAttnParams& p, c
     w.rp = (w.b - w.e * pl.R) * pl.per.d + w.r;
     return w;
 }
+// where row r of entry e (of B) and KV head hk has its partial result of the first of ns splits
+__device__ __forceinline__ long long ca_prow(const CaPlan& pl, int own, int r, int B, int e, int hk, int ns) {
+    const int blk = r >> pl.mtl;
+    const long long it = (((long long)blk * B + e) * pl.Hkv + hk) * ns;
+    return (own ? (long long)pl.items_p * pl.sp + it * pl.so : it * pl.sp) + (r - (blk << pl.mtl));
+}
 template <int D, typename T>
 __device__ __forceinline__ void ca_join_store(const SmxCachedAttnParams& p, const CaJoinRow& w, int dl, float m, float l, float o[4]) {
     T* out = reinterpret_cast<T*>(p.o) + w.b * p.o_bs + w.t * p.o_ts + w.h * p.o_hs + dl;
@@ -611,7 +618,7 @@ __device__ __forceinline__ void ca_join_store(const SmxCachedAttnParams& p, cons
 // O = sum over the splits of both parts, in a fixed order: JW waves per (row, head, query), D / 4 lanes per split.  A lane's loads depend on nothing but
 // the weights, and with four waves even 64 splits are four (D = 128: eight) of them.
 template <int D, int JW, typename T>
-__global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, CaPlan pl, int mt16) {
+__global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, CaPlan pl) {
     enum { LD = D / 4, NG = 64 / LD * JW };
     const int lane = threadIdx.x & 63, tid = JW == 4 ? threadIdx.x : lane;
     const int id = JW == 4 ? blockIdx.x : blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -623,13 +630,13 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
         const SmxKVCache& c = part ? p.own : p.pre;
         if (!c.k) continue;
         const int ns = part ? pl.nso : pl.nsp, e = part ? w.b : w.e, r = part ? w.r : w.rp;
-        const long long it = (part ? pl.items_p : 0) + (((long long)(r / mt16) * c.B + e) * pl.Hkv + w.hk) * ns;
-        const float* po = pl.po + (it * mt16 + r % mt16) * D + dl;
-        const long long step = (long long)mt16 * D;
+        const int step = part ? pl.so : pl.sp;                  // partial rows from one split to the next
+        const long long r0 = ca_prow(pl, part, r, c.B, e, w.hk, ns);
+        const float* po = pl.po + r0 * D + dl;
         // at most 64 splits: a lane holds one's maximum and sum
         float ms = CA_LOWEST, ls = 0.f;
         if (lane < ns) {
-            const float2 q = *reinterpret_cast<const float2*>(pl.pml + 2 * ((it + lane) * mt16 + r % mt16));
+            const float2 q = *reinterpret_cast<const float2*>(pl.pml + 2 * (r0 + (long long)lane * step));
             ms = q.x;
             ls = q.y;
         }
@@ -642,7 +649,7 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
         for (int s0 = 0; s0 < ns; s0 += 4 * NG) {
             float4 q[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const float4*>(po + min(s0 + NG * u + grp, ns - 1) * step);
+            for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const float4*>(po + (long long)min(s0 + NG * u + grp, ns - 1) * step * D);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int s = s0 + NG * u + grp;
@@ -670,13 +677,12 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
 
 // The same where each part has one split (prefixes and own keys that are both short): D / 4 lanes per row and nothing to pass between them.
 template <int D, typename T>
-__global__ __launch_bounds__(256) void attn_cached_join2(SmxCachedAttnParams p, CaPlan pl, int mt16) {
+__global__ __launch_bounds__(256) void attn_cached_join2(SmxCachedAttnParams p, CaPlan pl) {
     enum { LD = D / 4 };
     const int id = blockIdx.x * (256 / LD) + threadIdx.x / LD, dl = threadIdx.x % LD * 4;
     if (id >= p.B * p.H * p.Tq) return;
     const CaJoinRow w = ca_join_row(p, pl, id);
-    const long long ia = (((long long)(w.rp / mt16) * p.pre.B + w.e) * pl.Hkv + w.hk) * mt16 + w.rp % mt16;
-    const long long ib = (pl.items_p + ((long long)(w.r / mt16) * p.own.B + w.b) * pl.Hkv + w.hk) * mt16 + w.r % mt16;
+    const long long ia = ca_prow(pl, 0, w.rp, p.pre.B, w.e, w.hk, 1), ib = ca_prow(pl, 1, w.r, p.own.B, w.b, w.hk, 1);
     const float2 qa = *reinterpret_cast<const float2*>(pl.pml + 2 * ia), qb = *reinterpret_cast<const float2*>(pl.pml + 2 * ib);
     const float4 a = *reinterpret_cast<const float4*>(pl.po + ia * D + dl), c = *reinterpret_cast<const float4*>(pl.po + ib * D + dl);
     const float m = fmaxf(qa.x, qb.x);

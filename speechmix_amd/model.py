@@ -572,11 +572,11 @@ class SpeechMixEED(nn.Module):
         B, S = ids.shape
         return self.engine.lm_encode(None, ids.to(self.device).reshape(-1).contiguous(), B, S), B, S
 
-    def _decode_options(self, num_return_sequences, do_sample, temperature, kv_cache, assistant_model, num_assistant_tokens, generator):
+    def _decode_options(self, max_length, num_return_sequences, do_sample, temperature, kv_cache, assistant_model, num_assistant_tokens, generator):
         """Checks of generate's options -> True when the plain greedy loop serves them."""
         from . import decoding
         decoding.cache_format(kv_cache, self.compute_dtype)
-        if int(num_return_sequences) != num_return_sequences or num_return_sequences < 1:
+        if not isinstance(num_return_sequences, int) or num_return_sequences < 1:
             raise ValueError(f"num_return_sequences must be a positive number, got {num_return_sequences!r}")
         if num_return_sequences > 1 and not do_sample:
             raise ValueError("num_return_sequences > 1 needs do_sample=True (greedy rows would all be the same)")
@@ -590,9 +590,12 @@ class SpeechMixEED(nn.Module):
             a, t = assistant_model.decoder_model.config, self.decoder_model.config
             if (a.vocab_size, a.eos_token_id, a.decoder_start_token_id) != (t.vocab_size, t.eos_token_id, t.decoder_start_token_id):
                 raise ValueError("assistant_model must share the vocabulary and its eos / start ids")
-            if not 1 <= num_assistant_tokens <= 64:
+            if not isinstance(num_assistant_tokens, int) or not 1 <= num_assistant_tokens <= 64:
                 raise ValueError(f"num_assistant_tokens must be 1 .. 64, got {num_assistant_tokens!r}")
-        return not do_sample and kv_cache is None and assistant_model is None
+        plain = not do_sample and kv_cache is None and assistant_model is None
+        if not plain and max_length is not None and int(max_length) < 1:
+            raise ValueError(f"max_length must be at least 1 with these options, got {max_length!r}")
+        return plain
 
     def _cached_decode(self, enc, B, S, max_length, num_return_sequences, do_sample, temperature, kv_cache, assistant_model, assistant_enc,
                        num_assistant_tokens, generator):
@@ -628,7 +631,7 @@ class SpeechMixEED(nn.Module):
         are kept once for all its rows.  assistant_model: a smaller model of the same vocabulary whose decoder drafts num_assistant_tokens
         tokens at a time for this one to verify - the same tokens (greedy) or the same distribution (sampled) in fewer steps."""
         args = (num_return_sequences, do_sample, temperature, kv_cache, assistant_model, num_assistant_tokens, generator)
-        plain = self._decode_options(*args)
+        plain = self._decode_options(max_length, *args)
         enc, B, S = self._speech_encode(input_values)
         if plain:
             return self._greedy(enc, B, S, max_length)
@@ -641,7 +644,7 @@ class SpeechMixEED(nn.Module):
         """LM-only decoding of token ids [B, S] - what `create_self_decoder_input` loops over to make labels (ref:train.py:18-34:
         decoder_length = max(config.max_length, len(input)); stop at eos).  The options are `generate`'s."""
         args = (num_return_sequences, do_sample, temperature, kv_cache, assistant_model, num_assistant_tokens, generator)
-        plain = self._decode_options(*args)
+        plain = self._decode_options(max_length, *args)
         ids = torch.as_tensor(input_ids)
         if ids.dim() == 1:
             ids = ids[None]

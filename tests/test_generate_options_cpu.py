@@ -27,11 +27,20 @@ def test_refused_options(model, kw, err):
             call()
 
 
+@pytest.mark.parametrize("kw", [dict(max_length=0, kv_cache="fp8"), dict(max_length=-1, do_sample=True), dict(num_return_sequences=2.0, do_sample=True)])
+def test_refused_lengths_and_counts(model, kw):
+    for call in (lambda: model.generate(torch.zeros(1, 8000), **kw), lambda: model.generate_from_text(torch.zeros(1, 4, dtype=torch.int64), **kw)):
+        with pytest.raises(ValueError, match="max_length|num_return_sequences"):
+            call()
+
+
 def test_refused_assistants(model):
     other = SpeechMixEED(ENC, dict(LM, vocab_size=51), down_scale=2)
     with pytest.raises(ValueError, match="vocabulary"):
         model.generate(torch.zeros(1, 8000), assistant_model=other)
     same = SpeechMixEED(ENC, LM, down_scale=2)
+    with pytest.raises(ValueError, match="num_assistant_tokens"):
+        model.generate(torch.zeros(1, 8000), assistant_model=same, num_assistant_tokens=2.0)
     for n in (0, 65):
         with pytest.raises(ValueError, match="num_assistant_tokens"):
             model.generate(torch.zeros(1, 8000), assistant_model=same, num_assistant_tokens=n)

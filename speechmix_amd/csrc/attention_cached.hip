@@ -109,8 +109,9 @@ static int ca_cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 #define CA_SHORT 256          // keys of a cache that one wave takes
 // Splits of `cap` keys for `base` workgroups: up to `want` workgroups.  A split costs the second launch (4 us) and its partial rows, so it has to take
 // at least 512 keys (256 where few workgroups share the chip), and 2 048 where the rows alone already give it a workgroup per CU (32 x 16 heads x 777 keys: one launch 13 us,
-// two splits 14 + 4; 16 x 16 heads x 8 192 int8 keys: 84 us unsplit, 52 in four).
-static int ca_splits(long long base, int cap, long long want) {
+// two splits 14 + 4; 16 x 16 heads x 8 192 int8 keys: 84 us unsplit, 52 in four).  Up to `one` keys are not split at all.
+static int ca_splits(long long base, int cap, long long want, int one) {
+    if (cap <= one) return 1;
     const long long n = want / base, most = ca_cdiv(cap, base >= 256 ? 2048 : base >= 64 ? 512 : 256);
     const long long m = n < most ? n : most;
     return (int)(m < 1 ? 1 : m > 64 ? 64 : m);
@@ -131,10 +132,14 @@ static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, bool all1, CaPlan& 
     const long long want = mt == 1 && m.D == 64 ? 1024 : 512;
     // a wave per item where there are many items of few keys: a workgroup's other three waves would have nothing to do (16 384 rows and heads of
     // 43 keys behind prefixes: 151 us with a workgroup each, 55 so)
+    // one part of one tile of rows per item: what a single launch gets through sooner than two (16 heads of 64, 300 keys: 4.9 us for 7.4, 777: 7.2 for
+    // 7.5, 1 000: 8.2 for 7.6; 192 of them, 1 000 keys: 9.3 for 11.8; 16 heads of 128, 500 keys: 8.2 for 8.6, 777: 11.4 for 8.6; 192, 1 000 keys: 15.2 for 16.0)
+    const long long b1 = p.own.k ? bo : bp;
+    const int one = mt > 1 || (p.own.k && p.pre.k) ? 0 : m.D == 64 ? (b1 >= 64 ? 1024 : 768) : b1 >= 128 ? 1024 : 512;
     pl.single = all1 ? 2 : p.own.k && ro <= 16 && p.own.cap <= CA_SHORT && bo > 512;
-    pl.nso = !p.own.k ? 0 : pl.single ? 1 : ca_splits(bo, p.own.cap, want);
+    pl.nso = !p.own.k ? 0 : pl.single ? 1 : ca_splits(bo, p.own.cap, want, one);
     const long long left = want - (pl.single ? 0 : bo * pl.nso);        // (those of short caches are soon gone)
-    pl.nsp = !p.pre.k ? 0 : all1 ? 1 : ca_splits(bp, p.pre.cap, left > want / 2 ? left : want / 2);
+    pl.nsp = !p.pre.k ? 0 : all1 ? 1 : ca_splits(bp, p.pre.cap, left > want / 2 ? left : want / 2, one);
     pl.nso_ = ca_divisor(pl.nso > 0 ? pl.nso : 1);
     pl.nsp_ = ca_divisor(pl.nsp > 0 ? pl.nsp : 1);
     pl.items_p = (int)(bp * pl.nsp);

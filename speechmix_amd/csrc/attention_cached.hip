@@ -132,10 +132,12 @@ static void ca_plan_mt(const SmxCachedAttnParams& p, int mt, bool all1, CaPlan& 
     const long long want = mt == 1 && m.D == 64 ? 1024 : 512;
     // a wave per item where there are many items of few keys: a workgroup's other three waves would have nothing to do (16 384 rows and heads of
     // 43 keys behind prefixes: 151 us with a workgroup each, 55 so)
-    // one part of one tile of rows per item: what a single launch gets through sooner than two (16 heads of 64, 300 keys: 4.9 us for 7.4, 777: 7.2 for
-    // 7.5, 1 000: 8.2 for 7.6; 192 of them, 1 000 keys: 9.3 for 11.8; 16 heads of 128, 500 keys: 8.2 for 8.6, 777: 11.4 for 8.6; 192, 1 000 keys: 15.2 for 16.0)
+    // What a single launch gets through sooner than two, one tile of rows per item (16 heads of 64, 300 keys: 4.9 us for 7.4, 777: 7.2 for 7.5,
+    // 1 000: 8.2 for 7.6; 192 of them, 1 000 keys: 9.3 for 11.8; 16 heads of 128, 500 keys: 8.2 for 8.6, 777: 11.4 for 8.6; 192, 1 000 keys: 15.2
+    // for 16.0); two parts are joined in any case, but sooner where each has one result (8 rows x 12 heads of 64, 30 keys behind 300 and 500: 6.9 and 7.8
+    // us for 8.8 and 8.8; heads of 128, 500 keys: 10.2 for 10.0; in items of 64 rows 15.6 for 14.2).
     const long long b1 = p.own.k ? bo : bp;
-    const int one = mt > 1 || (p.own.k && p.pre.k) ? 0 : m.D == 64 ? (b1 >= 64 ? 1024 : 768) : b1 >= 128 ? 1024 : 512;
+    const int one = mt > 1 ? 0 : p.own.k && p.pre.k ? (m.D == 64 ? 512 : 0) : m.D == 64 ? (b1 >= 64 ? 1024 : 768) : b1 >= 128 ? 1024 : 512;
     pl.single = all1 ? 2 : p.own.k && ro <= 16 && p.own.cap <= CA_SHORT && bo > 512;
     pl.nso = !p.own.k ? 0 : pl.single ? 1 : ca_splits(bo, p.own.cap, want, one);
     const long long left = want - (pl.single ? 0 : bo * pl.nso);        // (those of short caches are soon gone)

@@ -363,9 +363,10 @@ static int vf_pieces(const SmxVerifyParams& p) {
     return c < 2 ? 1 : c > VF_MAXC ? VF_MAXC : c;
 }
 
-// One launch for the greedy form where a workgroup gets through its rows in the time of the second launch: it reads 100 GB/s (1 row set of 5 x
-// 32 128: 8 us, in two launches 5.7 + 1.9 and 3 us of host time; 64 x 5 x 50 265: 10 against 15 + 4; 5 x 250 027: 12 + 2 in two).
-static bool vf_greedy_one(const SmxVerifyParams& p) { return (long long)(p.n + 1) * p.V <= 400000; }
+// One launch for the greedy form of little work: two are always sooner on the GPU, but cost the caller 3 us of host time.  One set of 5 rows x 32 128:
+// 8.7 us by one workgroup (100 GB/s), 9.1 a call; 6.1 in two launches, 12.3 a call.  5 x 50 265: 11.5 and 5.7; 8 x 36 398: 17.0 and 5.9; 1 x 128 000:
+// 12.9 and 8.9; 64 sets of 8 x 36 398: 24.2 and 15.4.
+static bool vf_greedy_one(const SmxVerifyParams& p) { return p.V <= 65536 && (long long)(p.n + 1) * p.V <= 200000; }
 
 extern "C" long long smx_verify_draft_ws_bytes(const SmxVerifyParams* p) {
     if (vf_check(*p)) return SMX_EINVAL;

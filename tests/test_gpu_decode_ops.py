@@ -512,6 +512,23 @@ def test_verify_greedy_ties_logits_and_strides():
     assert a.tolist()[:2] == [0, 0] and tok.tolist()[:2] == [0, 0]
 
 
+def test_verify_greedy_ties_over_workgroups():
+    """The same where several workgroups share the rows: ties far apart, a row without a number, a row of the lowest values."""
+    from speechmix_amd import ops
+    V = 90001
+    t = torch.randn(3, 3, V, device="cuda", generator=_gen(10)) - 50
+    t[..., [90000, 45001, 30007]] = 1.0
+    ids = torch.tensor([[30007, 30007], [30007, 90000], [45001, 30007]], device="cuda")
+    a, tok = ops.verify_draft(t, ids)
+    assert a.tolist() == [2, 1, 0] and tok.tolist() == [30007, 30007, 30007]
+    t[0, 0] = float("-inf")
+    t[1, 0] = float("nan")
+    t[2, 0] = torch.finfo(torch.float32).min
+    t[2, 0, 70000] = -1e38
+    a, tok = ops.verify_draft(t, ids)
+    assert a.tolist() == [0, 0, 0] and tok.tolist() == [0, 0, 70000]
+
+
 def test_verify_distribution():
     """What comes out is distributed as the target whatever the draft: 60 000 draws of a five-token vocabulary, each frequency within five
     standard deviations."""

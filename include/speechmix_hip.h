@@ -317,7 +317,7 @@ int smx_kv_read(const SmxKVRowsParams* p, int dtype, hipStream_t stream);
  * (plen[g] tokens).  H a multiple of the caches' heads: query head h reads head h / (H / Hkv).  Prefix keys are visible to every query; with
  * `causal` query t sees own keys up to position klen - Tq + t.  Lengths are clamped to 0 .. cap; NULL lengths mean cap.  rel_bias [H, nrel]
  * adds rel_bias[h, clamp(qpos - kpos, 0, nrel - 1)] to the scaled score (positions count the prefix).  A query without a visible key gives
- * O = 0, lse = -inf.  ws: smx_attention_cached_ws_bytes bytes of device scratch (16-byte aligned), free to reuse once the launches are done;
+ * O = 0, lse = -inf; one whose scores hold a NaN (its own, or a visible token's under a NaN scale) gives NaN in both.  ws: smx_attention_cached_ws_bytes bytes of device scratch (16-byte aligned), free to reuse once the launches are done;
  * two launches that may overlap need one each. */
 typedef struct SmxCachedAttnParams {
     const void* q; void* o; float* lse; SmxKVCache own, pre; const int *klen, *plen; const float* rel_bias;

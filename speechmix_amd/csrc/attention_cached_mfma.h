@@ -85,9 +85,10 @@ __device__ __forceinline__ float ca_bias2(float b) {
     const float v = b * CA_LOG2E;
     return v < CA_LOWEST && b >= CA_LOWEST ? CA_LOWEST : v;
 }
-// log-sum-exp in natural units from a reference in log 2 units (a bias of the type's lowest value stays what it is)
+// log-sum-exp in natural units from a reference in log 2 units (a bias of the type's lowest value stays what it is).  A NaN never moves the
+// reference from where it starts, the lowest value: such a row is told by its sum.
 __device__ __forceinline__ float ca_lse(float m, float l) {
-    return l == 0.f ? -INFINITY : m == CA_LOWEST ? CA_LOWEST : fmaf(m, CA_LN2, logf(l));
+    return l == 0.f ? -INFINITY : m == CA_LOWEST && l == l ? CA_LOWEST : fmaf(m, CA_LN2, logf(l));
 }
 
 typedef __attribute__((ext_vector_type(4))) unsigned ca_u4;

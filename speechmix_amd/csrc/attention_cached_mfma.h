@@ -21,7 +21,17 @@
 #define CA_BK 32                  // keys per block and wave (64: more registers than they save instructions; two blocks ahead: spills)
 #define CA_LOG2E 1.44269504088896340736f
 #define CA_LN2 0.69314718055994530942f
-#define CA_BIG 65536.f            // a score may pass the reference by this factor before it moves
+#define CA_BIG 65536.f            // a probability may pass 1 by this factor before the reference moves
+// Range: sums of probabilities (of up to 2^16) times values shall overflow no sooner than those of the values themselves.
+//   8 bit: a probability times the scale keeps 16 (24) bits as two (three) bf16 numbers down to 2^-110, the smallest scale is 2^-126, and 2^16 times
+//   the largest does not fit.  Scales enter times CA_LIFT, from the first one past CA_LARGE on times CA_DROP; neither costs an ordinary one a bit.
+//   bf16: in a block with large values (told by the sum of a lane's squares) the reference moves at 1.
+// (Together 0.1 us a launch: 64 x 16 heads x 0 - 1 024 keys 17.0 -> 17.2 us, 16 x 33 queries x 16 x 700 keys 18.9 -> 19.4; a second pass over the keys where
+// the sums got large, in place of this, cost twice that.)
+#define CA_LIFT 0x1p32f
+#define CA_DROP 0x1p-30f
+#define CA_LARGE 0x1p28f
+#define CA_LARGE_SQ 0x1p120f
 #define CA_LOWEST (-3.402823466e38f)
 
 // waves per SIMD the registers are held to
@@ -265,7 +275,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
     unsigned one_lo = 0x0000bf80u, one_hi = 0xbf800000u;          // (-1, 0), (0, -1)
     asm("" : "+v"(one_lo), "+v"(one_hi));                       // (in registers: not every form of these constants means a pair)
     f32x4_t acc[MT][DT];
-    float m[MT], l[MT];
+    float m[MT], l[MT], lift = CA_LIFT;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         m[mt] = CA_LOWEST;
@@ -355,11 +365,33 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                             if ((x.v[a][r][q] & 0x7f800000u) == 0x7f800000u) x.v[a][r][q] &= 0xffffu;
                         }
         }
+        unsigned vs = 0;
+        if (FMT <= SMX_KV_INT8) {
+            if (__builtin_expect(__ballot(__uint_as_float(x.vs) > CA_LARGE) != 0 && lift == CA_LIFT, 0)) {
+                lift = CA_DROP;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[mt][d] *= CA_DROP / CA_LIFT;
+            }
+            vs = __float_as_uint(__uint_as_float(x.vs) * lift);
+        }
+        bool large = false;                             // (behind the lines above: hidden values that are not finite do not count)
+        if (FMT == SMX_KV_BF16) {
+            float sq = 0.f;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int q = 0; q < Blk::VW; ++q) sq = ca_dot2(x.v[a][r][q], x.v[a][r][q], sq);
+            large = __ballot(!(sq < CA_LARGE_SQ)) != 0;
+        }
         float vsc[2][4];
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) vsc[a][r] = FMT <= SMX_KV_INT8 ? ca_scale(x.vs, a, r) : 1.f;
+            for (int r = 0; r < 4; ++r) vsc[a][r] = FMT <= SMX_KV_INT8 ? ca_scale(vs, a, r) : 1.f;
         // ---- probabilities: one fused product and difference, one exponential.  A probability above 2^16 (also the first ever: the reference
         // starts at the lowest value) sends the row's wave back to the scores for a new reference.
         unsigned pf[MT][NP][4];
@@ -374,7 +406,7 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                     pr[a][r] = ca_exp2(fmaf(sc[mt][a][r], ksc[a][r], -m[mt]));
                     big = fmaxf(big, pr[a][r]);
                 }
-            if (__ballot(big > CA_BIG)) {
+            if (__ballot(big > (large ? 1.f : CA_BIG))) {
                 float mx = m[mt];
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
@@ -459,6 +491,22 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
             }
         }
         if (more) ca_load_v<FMT, D>(x, cv, j0 + WV * BK);
+    }
+    if (FMT <= SMX_KV_INT8) {
+        // (large values: what the reference lags behind is taken out of the sums as well, 1 / CA_DROP alone might not fit)
+        const bool low = lift != CA_LIFT;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float f = 1.f / CA_LIFT;
+            if (low) {
+                const bool lag = m[mt] != CA_LOWEST;    // (at the lowest value: none, and nothing to add to it)
+                f = lag ? 0x1p-16f / CA_DROP : 1.f / CA_DROP;
+                l[mt] *= lag ? 0x1p-16f : 1.f;
+                m[mt] += lag ? 16.f : 0.f;
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[mt][d] *= f;
+        }
     }
 
     if (WV == 1) {                                      // a wave has all of its rows: out of the registers

@@ -1260,6 +1260,14 @@ def _on_device(name, **tensors):
         _need(t.device.index == dev, f"{name}: {n} is on {t.device}, the current device is cuda:{dev}")
 
 
+def _no_history(name, *tensors):
+    """These operators have no backward: a call that autograd would have to remember is refused, not silently cut out of the graph."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward, and one of its tensors requires a gradient: call it under torch.no_grad(), or detach the tensor")
+
+
 def _disjoint(t):
     """No two index tuples of t name the same element (a broadcast or overlapping view cannot be written)."""
     reach = 0
@@ -1361,7 +1369,9 @@ def _kv_rows(name, cache, start, k, v, written):
 
 def kv_append(cache, k, v, start=0):
     """k, v [B, T, H, D] (fp32 / bf16, any strides with D contiguous) into the cache at positions start .. start + T - 1 (start: a number, or
-    int32 [B] on the device), quantised to the cache's format.  Rows that fall outside the capacity are dropped."""
+    int32 [B] on the device), quantised to the cache's format.  Rows that fall outside the capacity are dropped.  No backward: tensors that
+    require a gradient are refused while gradients are recorded (here and in the other two)."""
+    _no_history("kv_append", k, v, cache.k, cache.v)
     r = _kv_rows("kv_append", cache, start, k, v, False)
     if r:
         L.check(L.lib().smx_kv_append(C.byref(r[0]), r[1], _stream()), "smx_kv_append")
@@ -1369,6 +1379,7 @@ def kv_append(cache, k, v, start=0):
 
 def kv_read(cache, start, k, v):
     """The cache's values at positions start .. start + T - 1 into k, v [B, T, H, D] (fp32 / bf16).  Rows outside the capacity are left alone."""
+    _no_history("kv_read", k, v, cache.k, cache.v)
     r = _kv_rows("kv_read", cache, start, k, v, True)
     if r:
         L.check(L.lib().smx_kv_read(C.byref(r[0]), r[1], _stream()), "smx_kv_read")
@@ -1426,9 +1437,12 @@ def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel
     new ones included; None: the whole capacity) behind an optional `prefix` cache: entry g of it is shared by the B / prefix.B consecutive
     rows of group g (prefix_len int32 [groups]) and seen by all their queries.  cache = None: only the prefix.  `causal` orders the new
     tokens among themselves.  H may be a multiple of the caches' heads.  scale: D ** -0.5 unless given.  rel_bias fp32 [H, n]: bias by the
-    distance query - key, clamped to 0 .. n - 1.  A query that sees no key gives zeros and lse = -inf.  An inference operator: it has no backward.
+    distance query - key, clamped to 0 .. n - 1.  A query that sees no key gives zeros and lse = -inf, one whose scores hold a NaN gives NaN in both.
+    An inference operator: it has no backward, and refuses tensors that require a gradient while gradients are recorded.
     -> (out [B, Tq, H, D] of q's type, lse fp32 [B, H, Tq] or None)."""
     causal, scale = bool(causal), None if scale is None else float(scale)          # (values, not objects, in the signature)
+    if torch.is_grad_enabled():
+        _no_history("attention_cached", q, out, rel_bias, *(t for c in (cache, prefix) if c is not None for t in (c.k, c.v, c.ks, c.vs)))
     sig = (_sig(q), cache.signature if cache is not None else None, prefix.signature if prefix is not None else None, torch._C._cuda_getDevice(),
            _sig(klen), _sig(prefix_len), _sig(out), _sig(rel_bias), causal, scale)
     hit = _SIGNATURES.get(sig)

@@ -1,0 +1,54 @@
+"""Calls of the decoding operators that are refused or could be taken for another: gradients, views with unusual strides."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
+def test_a_call_that_would_lose_gradients_is_refused(fmt):
+    """No operator has a backward: with gradients recorded, tensors that require one are refused - also where a call of the same shapes has
+    passed before -, and accepted under no_grad or detached.  Drawing tokens has no gradient in the first place."""
+    from speechmix_amd import ops
+    c = ops.KVCache.empty(2, 2, 8, 64, fmt, "cuda")
+    x = torch.randn(2, 1, 2, 64, device="cuda")
+    rel = torch.randn(2, 4, device="cuda")
+    g = x.clone().requires_grad_()
+    grel, dst = rel.clone().requires_grad_(), torch.empty_like(x).requires_grad_()      # (dst is written, the inputs stay)
+    ops.kv_append(c, x, x)
+    want, _ = ops.attention_cached(x, c, rel_bias=rel, prefix=c)
+    ko, vo = torch.empty_like(x), torch.empty_like(x)
+    ops.kv_read(c, 0, ko, vo)
+    calls = [lambda: ops.attention_cached(g, c, rel_bias=rel, prefix=c), lambda: ops.attention_cached(x, c, rel_bias=grel, prefix=c),
+             lambda: ops.attention_cached(g * 2, None, prefix=c), lambda: ops.kv_append(c, g, x), lambda: ops.kv_append(c, x, g * 1), lambda: ops.kv_read(c, 0, dst, vo),
+             lambda: ops.attention_cached(x, c, out=g * 1)]
+    if fmt == "bf16":
+        grown = ops.KVCache(c.k.clone().requires_grad_(), c.v, fmt=fmt)
+        calls += [lambda: ops.attention_cached(x, grown), lambda: ops.attention_cached(x, None, prefix=grown), lambda: ops.kv_append(grown, x, x)]
+    for i, call in enumerate(calls):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+            raise AssertionError(f"call {i} was not refused")
+        with torch.no_grad():
+            call()
+    ops.kv_append(c, x, x)
+    with torch.no_grad():
+        assert torch.equal(ops.attention_cached(g, c, rel_bias=grel, prefix=c)[0], want)
+    assert torch.equal(ops.attention_cached(g.detach(), c, rel_bias=grel.detach(), prefix=c)[0], want)
+    p = torch.softmax(torch.randn(2, 1, 9, device="cuda"), -1).requires_grad_()
+    assert ops.verify_draft(p, torch.empty(2, 0, dtype=torch.int64, device="cuda"), None, torch.rand(2, 1, device="cuda"))[1].shape == (2,)
+
+
+@pytest.mark.parametrize("lm", ["bart", "t5"])
+def test_a_decoder_steps_while_gradients_are_recorded(lm):
+    """What CachedDecoder hands to the operators never requires a gradient, whoever calls it."""
+    from speechmix_amd.decoding import CachedDecoder
+    from tests.test_gpu_generate_options import BART, T5, _model, _wave
+    model = _model(BART if lm == "bart" else T5, "bf16")
+    with torch.no_grad():
+        enc, B, S = model._speech_encode(_wave(2))
+    assert torch.is_grad_enabled()
+    dec = CachedDecoder(model.engine, enc, B, S, 1, 8, "fp8")
+    for _ in range(3):
+        logits = dec.step(torch.full((B, 1), 5, dtype=torch.int64, device=model.device))
+    assert not logits.requires_grad

@@ -61,10 +61,10 @@ class CachedDecoder:
         self.use_graphs = eng.dev.type == "cuda" and eng.dt == BF16 and os.environ.get("SMX_DECODE_GRAPH", "1") != "0"
         self.graphs, self.warm = {}, set()
         self.rel = None
-        if self.t5:            # row `capacity - 1` of the bias sees every distance: [H, capacity], indexed by query - key
-            rel = eng._t5_bias("decoder", capacity, capacity)[0][:, capacity - 1].flip(-1)
-            # (the last bucket holds every distance from relative_attention_max_distance on: the operator clamps to the table's end)
-            self.rel = rel[:, :min(capacity, lc.relative_attention_max_distance + 1)].contiguous()
+        if self.t5:            # [H, n], indexed by query - key: what the last of n queries sees.  The last bucket holds every distance from
+            # relative_attention_max_distance on, and the operator clamps to the table's end: no more than that, whatever the capacity
+            n = min(capacity, lc.relative_attention_max_distance + 1)
+            self.rel = eng._t5_bias("decoder", 1, n, first=n - 1)[0][:, 0].flip(-1).contiguous()
         else:
             self.max_pos = st.offsets[self.pd + "embed_positions.weight"][2][0] - 1
         self.own = [ops.KVCache.empty(self.N, self.H, capacity, self.hd, self.fmt, eng.dev) for _ in self.names]

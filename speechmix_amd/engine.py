@@ -1716,17 +1716,17 @@ class Engine:
         if lo < 0 or hi >= V:
             raise IndexError(f"{what}: token id out of range [0, {V}) (min {lo}, max {hi})")
 
-    def _t5_bias(self, side, Tq, Tk):
-        """Relative-position bias [H, Tq, Tk] fp32 (TF:models/t5/modeling_t5.py:216-279).  Bucket indices are
-        integer host work; the gather from the [buckets, H] table is a pure index op."""
+    def _t5_bias(self, side, Tq, Tk, first=0):
+        """Relative-position bias [H, Tq, Tk] fp32 of the queries at `first` .. first + Tq - 1 (TF:models/t5/modeling_t5.py:216-279).
+        Bucket indices are integer host work; the gather from the [buckets, H] table is a pure index op."""
         lc = self.lc
         name = f"{self.lp}{side}.block.0.layer.0.SelfAttention.relative_attention_bias.weight"
         nb, md = lc.relative_attention_num_buckets, lc.relative_attention_max_distance
-        ck = ("_t5_buckets", side, Tq, Tk)
+        ck = ("_t5_buckets", side, Tq, Tk, first)
         if ck in self._persist:                     # (cached on the device: no host-to-device copy inside a step)
             buckets = self._persist[ck]
             return self.P(name)[buckets].permute(2, 0, 1).contiguous(), buckets
-        ctx = torch.arange(Tq)[:, None]
+        ctx = torch.arange(first, first + Tq)[:, None]
         mem = torch.arange(Tk)[None, :]
         rel = mem - ctx
         bidir = side == "encoder"

@@ -52,3 +52,21 @@ def test_a_decoder_steps_while_gradients_are_recorded(lm):
     for _ in range(3):
         logits = dec.step(torch.full((B, 1), 5, dtype=torch.int64, device=model.device))
     assert not logits.requires_grad
+
+
+def test_a_decoder_keeps_no_table_per_capacity():
+    """T5: the distance bias of a decoder of any capacity is the last row of the full table, and what the engine remembers for it is one row of at
+    most relative_attention_max_distance + 1 distances, not a square of the capacity."""
+    from speechmix_amd.decoding import CachedDecoder
+    from tests.test_gpu_generate_options import T5, _model, _wave
+    model = _model(T5, "bf16")
+    eng = model.engine
+    with torch.no_grad():
+        enc, B, S = model._speech_encode(_wave(2))
+        size = lambda: sum(t.numel() for k, t in eng._persist.items() if isinstance(k, tuple) and k[:2] == ("_t5_buckets", "decoder"))
+        before = size()
+        rels = {n: CachedDecoder(eng, enc, B, S, 1, n, "fp8").rel for n in (1, 2, 31, 128, 129, 130, 300, 512)}
+        assert size() - before <= 8 * 129
+        for n, rel in rels.items():
+            full = eng._t5_bias("decoder", n, n)[0][:, n - 1].flip(-1)
+            assert torch.equal(rel, full[:, :129]) and (n <= 129 or (full[:, 129:] == rel[:, -1:]).all())

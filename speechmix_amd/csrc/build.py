@@ -7,6 +7,7 @@ next to the package so it travels to the GPU box with the source snapshot.
 """
 import concurrent.futures as cf
 import os
+import shlex
 import subprocess
 import sys
 
@@ -25,11 +26,32 @@ if os.environ.get("SMX_PP_LAB"):      # ablation variants of the ping-pong GEMM 
     FLAGS.append("-DSMX_PP_LAB")
 
 
-def _newer(src, dst, deps):
+def command(src, obj):
+    """The compile command of one source."""
+    # SMX_TU: the file's stem - names the translation unit's step-key word (smx_common.h)
+    return (["hipcc"] + FLAGS + (NO_PK if os.path.basename(src) in NO_PK_FILES else [])
+            + ["-DSMX_TU=" + os.path.basename(src)[:-4], "-I", HERE, "-c", src, "-o", obj])
+
+
+def _line(cmd):
+    """A command as it is kept beside its object: the same wherever the tree stands."""
+    return shlex.join(cmd).replace(HERE, ".")
+
+
+def _stale(dst, deps, cmd=None):
+    """Is dst missing, older than one of deps, or made by another command?  (A command stands beside its object: flags that change - here or
+    through SMX_DEFS - leave no file newer.)"""
     if not os.path.exists(dst):
         return True
     t = os.path.getmtime(dst)
-    return any(os.path.getmtime(d) > t for d in [src] + deps)
+    if any(os.path.getmtime(d) > t for d in deps):
+        return True
+    if cmd is None:
+        return False
+    if not os.path.exists(dst + ".cmd"):
+        return True
+    with open(dst + ".cmd") as f:
+        return f.read() != _line(cmd)
 
 
 def build(force=False, verbose=True):
@@ -42,14 +64,16 @@ def build(force=False, verbose=True):
     for s in srcs:
         src = os.path.join(HERE, s)
         obj = os.path.join(OBJ, s.replace(".hip", ".o"))
-        if force or _newer(src, obj, hdrs):
+        if force or _stale(obj, [src] + hdrs, command(src, obj)):
             jobs.append((src, obj))
 
     def cc(job):
         src, obj = job
-        # SMX_TU: the file's stem - names the translation unit's step-key word (smx_common.h)
-        cmd = ["hipcc"] + FLAGS + (NO_PK if os.path.basename(src) in NO_PK_FILES else []) + ["-DSMX_TU=" + os.path.basename(src)[:-4], "-I", HERE, "-c", src, "-o", obj]
+        cmd = command(src, obj)
         r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode == 0:
+            with open(obj + ".cmd", "w") as f:
+                f.write(_line(cmd))
         return src, r.returncode, r.stdout + r.stderr
 
     if jobs:
@@ -61,7 +85,7 @@ def build(force=False, verbose=True):
                     sys.stderr.write(log)
                     raise RuntimeError(f"hipcc failed on {src}")
     objs = [os.path.join(OBJ, s.replace(".hip", ".o")) for s in srcs]
-    if jobs or not os.path.exists(OUT):
+    if jobs or _stale(OUT, objs):
         cmd = ["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT] + objs
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:

@@ -12,11 +12,14 @@ import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SRC = os.path.join(ROOT, "speechmix_amd", "csrc")
+sys.path.insert(0, SRC)
+import build  # noqa: E402
 
 
 def one(f):
-    asm = subprocess.run(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=fast", "-I", SRC, "-S",
-                          "--cuda-device-only", os.path.join(SRC, f), "-o", "-"], capture_output=True, text=True, check=True).stdout
+    cmd = build.command(os.path.join(SRC, f), "-")             # (with the flags of the library)
+    cmd[cmd.index("-c")] = "-S"
+    asm = subprocess.run(cmd + ["--cuda-device-only"], capture_output=True, text=True, check=True).stdout
     out = {}
     for m in re.finditer(r"\.amdhsa_kernel (\S+)(.*?)\.end_amdhsa_kernel", asm, flags=re.S):
         name, body = m.group(1), m.group(2)

@@ -7,7 +7,7 @@
 // instead of ever being stored; the only large traffic is the channels-last activation [B, T0, C] (32.8 MB / clip in
 // bf16), written once (forward) and read twice (backward).  What is left is VALU work - 10 FMAs + GroupNorm + GELU per
 // output element - so the kernels are built for the vector unit:
-//   * thread <-> one PAIR of channels, every op a packed-fp32 instruction (v_pk_fma_f32: two channels per issue);
+//   * thread <-> one PAIR of channels: two independent chains per thread;
 //     the whole block walks the same time steps, so the waveform window is an LDS broadcast;
 //   * exact tap count (template K = 10; a zero-padded 16-tap instance covers other kernels);
 //   * 20 weight + 20 gradient-accumulator registers per thread instead of 256: high occupancy, no spills;

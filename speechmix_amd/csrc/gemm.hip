@@ -394,7 +394,7 @@ __device__ __forceinline__ void epilogue_staged_fast(const SmxGemmParams& p, f32
                     for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], p.alpha, bs[e]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) {          // packed fp32: two columns per instruction
+                    for (int e = 0; e < 8; e += 2) {          // two columns at a time
                         const smx_f2 r = __builtin_elementwise_fma((smx_f2){x[e], x[e + 1]}, al2, (smx_f2){bs[e], bs[e + 1]});
                         x[e] = r[0];
                         x[e + 1] = r[1];

@@ -32,6 +32,13 @@ struct SmxNormParams {
     unsigned drop_seed;
 };
 
+// A product that is rounded before it is added, never fused with the sum.  Left to itself the compiler does one or the other as its vectoriser pleases, and
+// every recorded result behind a norm would change with its flags; so each sum of a row says here which of the two it is.
+__device__ __forceinline__ float rounded(float product) {
+    asm("" : "+v"(product));                            // (no instruction)
+    return product;
+}
+
 // One wave per row, blocks persistent over the rows (grid = one resident round of the chip, smx_norm_fwd): gamma / beta are
 // loaded once per wave instead of once per row, and a wave's next row is requested while it finishes the current one.
 template <typename T>
@@ -87,7 +94,7 @@ __global__ __launch_bounds__(256, LN_FWD_BLOCKS_PER_CU) void norm_fwd_kernel(Smx
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float d = v[j][e] - mean;
-                    q += d * d;
+                    q += rounded(d * d);
                 }
             }
         }
@@ -183,11 +190,11 @@ __global__ __launch_bounds__(256) void norm_bwd_dx_kernel(SmxNormBwdParams p) {
                 if (p.drop_p > 0.f)
                     d *= smx_drop_mul(p.drop_seed, (unsigned)(row * p.D + c + e), smx_thresh24(p.drop_p), 1.0f / (1.0f - p.drop_p));
                 if (ACT) d *= act_grad(xhat * gm[e] + bt[e], p.act);
-                const float gg = d * gm[e];
+                const float gg = rounded(d * gm[e]);
                 xh[j][e] = xhat;
                 g[j][e] = gg;
                 s1 += gg;
-                s2 += gg * xhat;
+                s2 += rounded(gg * xhat);
             }
         }
     }
@@ -204,7 +211,7 @@ __global__ __launch_bounds__(256) void norm_bwd_dx_kernel(SmxNormBwdParams p) {
             if (dres) load8(dres + c, r);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                o[e] = (g[j][e] - s1 - xh[j][e] * s2) * rstd;
+                o[e] = fmaf(-s2, xh[j][e], g[j][e] - s1) * rstd;
                 if (dpos) atomicAdd(dpos + c + e, o[e]);
                 if (dres) o[e] += r[e];
             }
@@ -360,13 +367,13 @@ __global__ __launch_bounds__(256, PR == 1 ? LN_BLOCKS_PER_CU : 1) void norm_bwd_
                     d *= smx_drop_mul(p.drop_seed, (unsigned)(row * p.D + (lane + 64 * j) * 8 + e), smx_thresh24(p.drop_p),
                                       1.0f / (1.0f - p.drop_p));
                 if (ACT) d *= act_grad(xhat * gm[j][e] + bt[j][e], p.act);
-                dg[j][e] += d * xhat;
+                dg[j][e] += rounded(d * xhat);
                 db[j][e] += d;
-                const float gg = d * gm[j][e];
+                const float gg = rounded(d * gm[j][e]);
                 xv[r][j][e] = xhat;               // (reuse the staging registers: xhat and the scaled gradient)
                 dv[r][j][e] = gg;
                 s1 += gg;
-                s2 += gg * xhat;
+                s2 = fmaf(gg, xhat, s2);
             }
         s1 = p.rms ? 0.f : wave_sum(s1) * invD;
         s2 = wave_sum(s2) * invD;
@@ -382,7 +389,7 @@ __global__ __launch_bounds__(256, PR == 1 ? LN_BLOCKS_PER_CU : 1) void norm_bwd_
                     if (dres) load8(dres + c, rr);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        o[e] = (dv[r][j][e] - s1 - xv[r][j][e] * s2) * rstd[r];
+                        o[e] = fmaf(-s2, xv[r][j][e], dv[r][j][e] - s1) * rstd[r];
                         if (dpos) atomicAdd(dpos + c + e, o[e]);
                         if (dres) o[e] += rr[e];
                     }

@@ -105,8 +105,8 @@ __device__ __forceinline__ float act_grad(float x, int act) {
     return 1.f;
 }
 
-// ---- the same two functions on 8 values with packed fp32 math (v_pk_fma_f32 / v_pk_mul_f32 process two values per
-// instruction at full rate; the activation epilogues are VALU-bound).  erf(x/sqrt2) and the Gaussian pdf share ONE
+// ---- the same two functions on 8 values, pair by pair (the library is built without packed fp32 instructions, so a pair is two
+// independent scalar chains; the activation epilogues are VALU-bound).  erf(x/sqrt2) and the Gaussian pdf share ONE
 // exponential E = exp(-x^2/2): erf = 1 - poly(t) t E (A&S 7.1.26 at z = |x|/sqrt2), pdf = E / sqrt(2 pi).
 typedef __attribute__((ext_vector_type(2))) float smx_f2;
 #define SMX_PK(v) ((smx_f2){(v), (v)})

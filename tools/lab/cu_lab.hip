@@ -1,5 +1,5 @@
 // CU laboratory (not part of the product library): what one CU's LDS and LDS-DMA path deliver, alone and together.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 cu_lab.hip -o cu_lab
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops cu_lab.hip -o cu_lab
 // Every kernel runs one 160-KB workgroup per CU on all CUs and reports bytes per shader clock per CU (s_memtime) and
 // per wall second (HIP events).  Roles per wave:  R = ds_read_b128 stream (conflict-free, 16 reads per wait),
 // D = LDS-DMA stream (buffer_load_dwordx4 ... lds, `inflight` instructions kept outstanding), M = MFMA stream, - = idle.

@@ -6,7 +6,7 @@
 //   pat 2  lane >> 3 -> row, lane & 7 -> chunk          8 rows x 128 B  (8 lanes = one full line)
 //   pat 3  (lane & 7) | rows interleaved: lane & 7 -> row, lane >> 3 -> chunk   8 rows x 128 B, lanes of a row 8 apart
 //   pat 4  1 KB contiguous
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/lab/st_lab tools/lab/st_lab.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/lab/st_lab tools/lab/st_lab.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -343,27 +343,37 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                 for (int r = 0; r < 4; ++r) ksc[a][r] = 1.f;
         }
         if (more) ca_load_k<FMT, D>(x, cv, j0 + WV * BK);
-        bool odd = false;                               // bf16: a value that is not finite in a block of which some row must not see all
-        if (FMT == SMX_KV_BF16 && masked) {
-            bool bad = false;
+        // bf16: large values in the block; some that are not finite
+        bool large = false, odd = false;
+        if (FMT == SMX_KV_BF16) {
+            const auto squares = [&x]() {               // of this lane's values
+                float sq = 0.f;
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+                    for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int q = 0; q < Blk::VW; ++q)
-                        bad |= (x.v[a][r][q] & 0x7f80u) == 0x7f80u || (x.v[a][r][q] & 0x7f800000u) == 0x7f800000u;
-            odd = causal && __ballot(bad) != 0;
-            if (odd)                                    // (the product leaves them out; the rows that do see them get them below)
+                        for (int q = 0; q < Blk::VW; ++q) sq = ca_dot2(x.v[a][r][q], x.v[a][r][q], sq);
+                return sq;
+            };
+            large = __ballot(!(squares() < CA_LARGE_SQ)) != 0;
+            if (__builtin_expect(large, 0)) {
+                // The product leaves those that are not finite out (a hidden one, or the zero that a probability's second part may be, would make NaN of
+                // them); the rows that see them get them below.
+                bool bad = false;
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int q = 0; q < Blk::VW; ++q) {
-                            if ((x.v[a][r][q] & 0x7f80u) == 0x7f80u) x.v[a][r][q] &= 0xffff0000u;
-                            if ((x.v[a][r][q] & 0x7f800000u) == 0x7f800000u) x.v[a][r][q] &= 0xffffu;
+                            unsigned& u = x.v[a][r][q];
+                            if ((u & 0x7f80u) == 0x7f80u) { u &= 0xffff0000u; bad = true; }
+                            if ((u & 0x7f800000u) == 0x7f800000u) { u &= 0xffffu; bad = true; }
                         }
+                odd = __ballot(bad) != 0;
+                large = __ballot(!(squares() < CA_LARGE_SQ)) != 0;
+            }
         }
         unsigned vs = 0;
         if (FMT <= SMX_KV_INT8) {
@@ -375,17 +385,6 @@ __device__ __forceinline__ void ca_body(const SmxCachedAttnParams& p, const CaPl
                     for (int d = 0; d < DT; ++d) acc[mt][d] *= CA_DROP / CA_LIFT;
             }
             vs = __float_as_uint(__uint_as_float(x.vs) * lift);
-        }
-        bool large = false;                             // (behind the lines above: hidden values that are not finite do not count)
-        if (FMT == SMX_KV_BF16) {
-            float sq = 0.f;
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int q = 0; q < Blk::VW; ++q) sq = ca_dot2(x.v[a][r][q], x.v[a][r][q], sq);
-            large = __ballot(!(sq < CA_LARGE_SQ)) != 0;
         }
         float vsc[2][4];
 #pragma unroll
@@ -702,11 +701,13 @@ __global__ __launch_bounds__(256) void attn_cached_join(SmxCachedAttnParams p, C
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int s = s0 + NG * u + grp;
-                const float v = __shfl(fs, s & 63, 64), f = s < ns ? v : 0.f;
-                o[0] = fmaf(q[u].x, f, o[0]);
-                o[1] = fmaf(q[u].y, f, o[1]);
-                o[2] = fmaf(q[u].z, f, o[2]);
-                o[3] = fmaf(q[u].w, f, o[3]);
+                const float f = __shfl(fs, s & 63, 64);
+                if (s < ns) {                           // (an infinity times a weight of zero is not nothing)
+                    o[0] = fmaf(q[u].x, f, o[0]);
+                    o[1] = fmaf(q[u].y, f, o[1]);
+                    o[2] = fmaf(q[u].z, f, o[2]);
+                    o[3] = fmaf(q[u].w, f, o[3]);
+                }
             }
         }
     }

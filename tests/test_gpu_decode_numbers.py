@@ -141,3 +141,38 @@ def test_large_values_under_a_bias_that_masks(fmt):
     V = R.values(c.v, c.vs, fmt)[0]
     tol = (300 + 64) * 2.0 ** -24 * V.abs().mean(1) + 2.0 ** -24 * V.mean(1).abs()
     assert ((o[0, 0].double().cpu() - V.mean(1)).abs() <= tol).all() and (lse == low).all()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f32"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128, 32])
+@pytest.mark.parametrize("B,H,cap,P,Tq,causal", [(3, 2, 1, 0, 1, False), (3, 2, 40, 0, 1, False), (3, 2, 300, 0, 1, True), (3, 2, 5000, 0, 1, True), (3, 2, 40, 0, 4, True), (3, 2, 40, 0, 33, False),
+                                                 (93, 6, 47, 0, 1, True), (6, 2, 40, 30, 2, True), (96, 6, 47, 20, 1, True), (6, 2, 0, 700, 1, False), (96, 8, 0, 60, 1, False)])
+def test_visible_values_that_are_not_finite(fmt, dtype, D, B, H, cap, P, Tq, causal):
+    """Caches that hold the values themselves may hold infinities and NaN: where a query sees one, that element of its output - and no other - is
+    the infinity or NaN that a positive probability makes of it."""
+    from speechmix_amd import ops
+    q = torch.randn(B, Tq, H, D, device="cuda", generator=_gen(3)).to(dtype)
+    kl = torch.tensor([max(cap - i, 1) for i in range(3)] * (B // 3), dtype=torch.int32, device="cuda") if cap else None
+    c = _rows(B, H, cap, D, fmt, 1) if cap else None
+    pre = _rows(B // 3, H, P, D, fmt, 2) if P else None
+    want, wl = ops.attention_cached(q, c, kl, causal=causal, prefix=pre, want_lse=True)
+    main, other = (c, pre) if cap else (pre, None)
+    main.v[0, 0, 0, 3], main.v[0, 0, 0, 4], main.v[0, 1, 0, 5] = float("inf"), -float("inf"), float("nan")
+    if main.cap > 6:
+        main.v[0, 0, 6, 3], main.v[0, 0, 5, 4] = float("inf"), float("inf")               # inf twice, inf and -inf
+    if other is not None:
+        other.v[0, 1, 7, 9] = float("inf")
+    got, gl = ops.attention_cached(q, c, kl, causal=causal, prefix=pre, want_lse=True)
+    assert torch.equal(gl, wl)
+    expect = want.clone().float()
+    for r in range(1 if cap else 3):                       # (a prefix: the rows of its first group)
+        for t in range(Tq):
+            seen = main.cap if not cap else int(kl[0]) if not causal else int(kl[0]) - Tq + t + 1
+            if seen > 0:
+                expect[r, t, 0, 3], expect[r, t, 0, 4], expect[r, t, 1, 5] = float("inf"), -float("inf") if seen <= 5 else float("nan"), float("nan")
+    if other is not None:
+        expect[:3, :, 1, 9] = float("inf")
+    same = torch.isfinite(expect)
+    assert torch.equal(got.float().nan_to_num(nan=7e30, posinf=8e30, neginf=9e30)[~same], expect.nan_to_num(nan=7e30, posinf=8e30, neginf=9e30)[~same])
+    assert torch.equal(got[same], want[same])

@@ -72,6 +72,13 @@ __global__ __launch_bounds__(256) void attn_cached_simple(SmxCachedAttnParams p)
     if (p.lse && lane == 0) p.lse[((long long)b * p.H + h) * p.Tq + t] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
+// The call as the kernels take it: the token stride of a cache of one token means nothing, but blocks of keys are addressed by it (what lies past the last
+// key must lie past the end of the buffer).
+static SmxCachedAttnParams ca_params(SmxCachedAttnParams p) {
+    for (SmxKVCache* c : {&p.own, &p.pre})
+        if (c->k && c->cap == 1) c->ts = c->D;
+    return p;
+}
 static int ca_check(const SmxCachedAttnParams& p, int dtype) {
     if (!p.q || !p.o || p.B <= 0 || p.Tq <= 0 || p.H <= 0 || (dtype != SMX_F32 && dtype != SMX_BF16)) return SMX_EINVAL;
     if (!p.own.k && !p.pre.k) return SMX_EINVAL;
@@ -193,11 +200,12 @@ static long long ca_prows(const CaPlan& pl) { return (long long)pl.items_p * pl.
 // bytes of workspace smx_attention_cached needs for these sizes (0: none)
 extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp, int dtype) {
     if (ca_check(*pp, dtype)) return SMX_EINVAL;
-    if (!ca_mfma_ok(*pp)) return 0;
+    const SmxCachedAttnParams p = ca_params(*pp);
+    if (!ca_mfma_ok(p)) return 0;
     CaPlan pl;
     long long items;
-    ca_plan(*pp, dtype, pl, items);
-    return pl.join ? ca_prows(pl) * ((pp->own.k ? pp->own.D : pp->pre.D) + 2) * 4 : 0;
+    ca_plan(p, dtype, pl, items);
+    return pl.join ? ca_prows(pl) * ((p.own.k ? p.own.D : p.pre.D) + 2) * 4 : 0;
 }
 
 #define CA_SIMPLE(FMT)                                                                                                                \
@@ -247,9 +255,9 @@ extern "C" long long smx_attention_cached_ws_bytes(const SmxCachedAttnParams* pp
 
 extern "C" int smx_attention_cached(const SmxCachedAttnParams* pp, int dtype, hipStream_t stream) {
     (void)hipGetLastError();
-    const SmxCachedAttnParams p = *pp;
-    const int rc = ca_check(p, dtype);
+    const int rc = ca_check(*pp, dtype);
     if (rc) return rc;
+    const SmxCachedAttnParams p = ca_params(*pp);
     const int fmt = p.own.k ? p.own.fmt : p.pre.fmt, D = p.own.k ? p.own.D : p.pre.D;
     if (ca_mfma_ok(p)) {
         CaPlan pl;

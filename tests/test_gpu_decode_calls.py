@@ -70,3 +70,33 @@ def test_a_decoder_keeps_no_table_per_capacity():
         for n, rel in rels.items():
             full = eng._t5_bias("decoder", n, n)[0][:, n - 1].flip(-1)
             assert torch.equal(rel, full[:, :129]) and (n <= 129 or (full[:, 129:] == rel[:, -1:]).all())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f32", "e4m3"])
+@pytest.mark.parametrize("ts", [0, 8, 64, 1 << 25])
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_token_stride_of_a_cache_of_one_token_means_nothing(fmt, ts, D):
+    """A dimension of one element may have any stride: nothing is read at it, also where the one token's values are not finite (whose product with a
+    hidden token's probability of zero would be NaN)."""
+    from speechmix_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(3)
+    want = ops.KVCache.empty(3, 2, 1, D, fmt, "cuda")
+    k, v = (torch.randn(3, 1, 2, D, device="cuda", generator=g) for _ in range(2))
+    ops.kv_append(want, k, v)
+    if fmt != "e4m3":
+        want.v[1, 0, 0, 40] = float("inf")
+    view = lambda t: t.as_strided(t.shape, (2 * D, D, ts, 1))
+    c = ops.KVCache(view(want.k), view(want.v), want.ks, want.vs, fmt=fmt)
+    q = torch.randn(3, 2, 2, D, device="cuda", generator=g).to(torch.bfloat16)
+    for kw in (dict(causal=False), dict(causal=True), dict(prefix=True)):
+        if "prefix" in kw:
+            a, b = (ops.attention_cached(q, None, prefix=x, want_lse=True) for x in (want, c))
+        else:
+            a, b = (ops.attention_cached(q, x, want_lse=True, **kw) for x in (want, c))
+        assert torch.equal(a[0].isnan(), b[0].isnan()) and torch.equal(a[0].nan_to_num(), b[0].nan_to_num()) and torch.equal(a[1], b[1])
+        if kw.get("causal", False) is False:
+            assert torch.equal(b[0].isnan().any(), torch.tensor(False, device="cuda"))
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    ops.kv_append(c, k * 2, v * 2)
+    ops.kv_read(want, 0, ko, vo)
+    assert (vo - 2 * v).abs().max() <= 2.0 ** -4 * 2 * v.abs().max()

@@ -122,3 +122,14 @@ def test_reference_quantisation_against_torch():
     assert s.item() == 1.0
     assert torch.equal(code[0].view(torch.uint8), x.to(torch.float8_e4m3fn).view(torch.uint8))
     assert torch.equal(R.values(code, s, "e4m3")[0], x.to(torch.float8_e4m3fn).double())
+
+
+def test_a_split_call_needs_its_workspace(lib):
+    """A row of 2^20 keys is split in every format that is split at all: it has a workspace, and none, a short or an unaligned one is refused."""
+    for fmt in (L.KV_E4M3, L.KV_INT8, L.KV_BF16):
+        p = L.CachedAttnParams(q=4096, o=4096, own=_cache(B=1, H=1, cap=1 << 20, fmt=fmt), B=1, Tq=1, H=1, scale=1.0)
+        n = lib.smx_attention_cached_ws_bytes(C.byref(p), 1)
+        assert n >= 2 * (64 + 2) * 4                   # at least two partial rows of 64 numbers, a maximum and a sum
+        for ws, size in ((4096, n - 1), (4104, n), (None, n), (4096, 0)):
+            p.ws, p.ws_bytes = ws, size
+            assert lib.smx_attention_cached(C.byref(p), 1, None) == -22

@@ -580,8 +580,8 @@ class SpeechMixEED(nn.Module):
             raise ValueError(f"num_return_sequences must be a positive number, got {num_return_sequences!r}")
         if num_return_sequences > 1 and not do_sample:
             raise ValueError("num_return_sequences > 1 needs do_sample=True (greedy rows would all be the same)")
-        if not (temperature > 0 and math.isfinite(temperature)):
-            raise ValueError(f"temperature must be positive and finite, got {temperature!r} (do_sample=False is the greedy limit)")
+        if not (1e-20 <= temperature and math.isfinite(temperature)):       # (below: logits / temperature would not fit fp32)
+            raise ValueError(f"temperature must be finite and at least 1e-20, got {temperature!r} (do_sample=False is the greedy limit)")
         if generator is not None and not do_sample:
             raise ValueError("generator without do_sample=True")
         if assistant_model is not None:
@@ -626,8 +626,8 @@ class SpeechMixEED(nn.Module):
         token, cut before eos): a row per clip, or num_return_sequences consecutive rows per clip.
 
         Greedy unless do_sample=True (from softmax(logits / temperature), with uniforms of `generator`, a torch.Generator on the model's
-        device).  kv_cache: "fp8" (e4m3 with a power-of-two scale per token and head) or "int8" keeps the decoder's self- and
-        cross-attention keys and values in one byte per element; "bf16" / "fp32" / None in the model's type.  The cross-attention keys of a clip
+        device; temperature at least 1e-20).  kv_cache: "fp8" (e4m3 with a power-of-two scale per token and head) or "int8" keeps the
+        decoder's self- and cross-attention keys and values in one byte per element; "bf16" / "fp32" in that type, None in the model's.  The cross-attention keys of a clip
         are kept once for all its rows.  assistant_model: a smaller model of the same vocabulary whose decoder drafts num_assistant_tokens
         tokens at a time for this one to verify - the same tokens (greedy) or the same distribution (sampled) in fewer steps."""
         args = (num_return_sequences, do_sample, temperature, kv_cache, assistant_model, num_assistant_tokens, generator)

@@ -53,3 +53,14 @@ def test_cache_formats():
     from speechmix_amd.decoding import cache_format
     assert cache_format(None, ops.BF16) == "bf16" and cache_format(None, ops.F32) == "f32"
     assert cache_format("fp8", ops.BF16) == "e4m3" and cache_format("int8", ops.F32) == "int8"
+
+
+@pytest.mark.parametrize("temperature", [1e-21, 1e-40, 5e-324, -1.0, float("inf")])
+def test_temperatures_that_leave_no_numbers_are_refused(model, temperature):
+    """Logits divided by a vanishing temperature are infinite, their probabilities NaN and the drawn token 0: refused."""
+    for call in (lambda: model.generate(torch.zeros(1, 8000), do_sample=True, temperature=temperature),
+                 lambda: model.generate_from_text(torch.zeros(1, 4, dtype=torch.int64), do_sample=True, temperature=temperature)):
+        with pytest.raises(ValueError, match="temperature"):
+            call()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):          # the lowest that is taken gets as far as the missing device
+        model.generate(torch.zeros(1, 8000), do_sample=True, temperature=1e-20)

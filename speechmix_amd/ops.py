@@ -1261,11 +1261,11 @@ def _on_device(name, **tensors):
 
 
 def _no_history(name, *tensors):
-    """These operators have no backward: a call that autograd would have to remember is refused, not silently cut out of the graph."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} has no backward, and one of its tensors requires a gradient: call it under torch.no_grad(), or detach the tensor")
+    """(While gradients are recorded.)  These operators have no backward: a call that autograd would have to remember is refused, not silently cut
+    out of the graph."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"{name} has no backward, and one of its tensors requires a gradient: call it under torch.no_grad(), or detach the tensor")
 
 
 def _disjoint(t):
@@ -1371,7 +1371,8 @@ def kv_append(cache, k, v, start=0):
     """k, v [B, T, H, D] (fp32 / bf16, any strides with D contiguous) into the cache at positions start .. start + T - 1 (start: a number, or
     int32 [B] on the device), quantised to the cache's format.  Rows that fall outside the capacity are dropped.  No backward: tensors that
     require a gradient are refused while gradients are recorded (here and in the other two)."""
-    _no_history("kv_append", k, v, cache.k, cache.v)
+    if torch.is_grad_enabled():
+        _no_history("kv_append", k, v, cache.k, cache.v)
     r = _kv_rows("kv_append", cache, start, k, v, False)
     if r:
         L.check(L.lib().smx_kv_append(C.byref(r[0]), r[1], _stream()), "smx_kv_append")
@@ -1379,7 +1380,8 @@ def kv_append(cache, k, v, start=0):
 
 def kv_read(cache, start, k, v):
     """The cache's values at positions start .. start + T - 1 into k, v [B, T, H, D] (fp32 / bf16).  Rows outside the capacity are left alone."""
-    _no_history("kv_read", k, v, cache.k, cache.v)
+    if torch.is_grad_enabled():
+        _no_history("kv_read", k, v, cache.k, cache.v)
     r = _kv_rows("kv_read", cache, start, k, v, True)
     if r:
         L.check(L.lib().smx_kv_read(C.byref(r[0]), r[1], _stream()), "smx_kv_read")
@@ -1442,7 +1444,11 @@ def attention_cached(q, cache, klen=None, out=None, causal=True, scale=None, rel
     -> (out [B, Tq, H, D] of q's type, lse fp32 [B, H, Tq] or None)."""
     causal, scale = bool(causal), None if scale is None else float(scale)          # (values, not objects, in the signature)
     if torch.is_grad_enabled():
-        _no_history("attention_cached", q, out, rel_bias, *(t for c in (cache, prefix) if c is not None for t in (c.k, c.v, c.ks, c.vs)))
+        _no_history("attention_cached", q, out, rel_bias)
+        if cache is not None:
+            _no_history("attention_cached", cache.k, cache.v, cache.ks, cache.vs)
+        if prefix is not None:
+            _no_history("attention_cached", prefix.k, prefix.v, prefix.ks, prefix.vs)
     sig = (_sig(q), cache.signature if cache is not None else None, prefix.signature if prefix is not None else None, torch._C._cuda_getDevice(),
            _sig(klen), _sig(prefix_len), _sig(out), _sig(rel_bias), causal, scale)
     hit = _SIGNATURES.get(sig)

@@ -317,8 +317,10 @@ int smx_kv_read(const SmxKVRowsParams* p, int dtype, hipStream_t stream);
  * (plen[g] tokens).  H a multiple of the caches' heads: query head h reads head h / (H / Hkv).  Prefix keys are visible to every query; with
  * `causal` query t sees own keys up to position klen - Tq + t.  Lengths are clamped to 0 .. cap; NULL lengths mean cap.  rel_bias [H, nrel]
  * adds rel_bias[h, clamp(qpos - kpos, 0, nrel - 1)] to the scaled score (positions count the prefix).  A query without a visible key gives
- * O = 0, lse = -inf; one whose scores hold a NaN (its own, or a visible token's under a NaN scale) gives NaN in both.  ws: smx_attention_cached_ws_bytes bytes of device scratch (16-byte aligned), free to reuse once the launches are done;
- * two launches that may overlap need one each. */
+ * O = 0, lse = -inf; one whose scores hold a NaN (its own, or a visible token's under a NaN scale) gives NaN in both.  Finite caches of any
+ * magnitude give finite outputs; 8-bit codes have to be finite (e4m3 has two that are not: smx_kv_append writes neither), values of the other
+ * formats need not be, and hidden ones never count.  ws: smx_attention_cached_ws_bytes bytes of device scratch (16-byte aligned), free to reuse
+ * once the launches are done; two launches that may overlap need one each. */
 typedef struct SmxCachedAttnParams {
     const void* q; void* o; float* lse; SmxKVCache own, pre; const int *klen, *plen; const float* rel_bias;
     long long q_bs, q_ts, q_hs, o_bs, o_ts, o_hs; void* ws; long long ws_bytes;
@@ -330,7 +332,8 @@ int smx_attention_cached(const SmxCachedAttnParams* p, int dtype, hipStream_t st
  * draft i is accepted while u_i * q_i(x_i) < p_i(x_i) (draft = NULL: q_i is 1 at x_i); the next token is drawn with u_n from
  * max(p_r - q_r, 0) at the first rejected draft r, from p when all are accepted or at an id outside 0 .. V - 1 (a shorter draft).  Drawn index:
  * the smallest whose running sum exceeds u_n times the total (64-bit sums).  n = 0 is plain sampling.  u = NULL: greedy, accepted while id ==
- * arg max (lowest index of ties; target may be logits).  n <= 64.  ws: smx_verify_draft_ws_bytes bytes (8-byte aligned). */
+ * arg max (lowest index of ties; target may be logits; a NaN is below everything, a row of nothing above -inf gives 0).  In the sampled form a
+ * NaN or a negative number weighs nothing.  n <= 64.  ws: smx_verify_draft_ws_bytes bytes (8-byte aligned). */
 typedef struct SmxVerifyParams {
     const float *target, *draft, *u; const long long* ids; int* accepted; long long* token; void* ws; long long ws_bytes;
     long long t_bs, t_ts, d_bs, d_ts, ids_bs, u_bs; int B, n, V, _pad;

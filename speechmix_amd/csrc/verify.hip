@@ -5,7 +5,8 @@
 //   all weights); sums in 64 bits - the borders of 50 000 intervals lie closer than 32-bit sums are sure of.
 // Bounds: a chain of dependent loads and scans, 5.4 us whatever the size (ids -> probabilities at the ids -> the row -> its sums -> the chosen segment
 // again), and what one CU reads (100 GB/s) of the one or two rows that count: 64 rows of 50 265 with four drafts 11 us, 256 rows without drafts 13 us.
-//   u = null: greedy - draft i is accepted while it equals arg max p_i (ties: the lowest index; target may then hold logits).
+//   u = null: greedy - draft i is accepted while it equals arg max p_i (ties: the lowest index; target may then hold logits; a NaN is below
+//   everything - a step whose logits broke draws the best of what is left, or 0).
 #include "smx_common.h"
 
 struct SmxVerifyParams {

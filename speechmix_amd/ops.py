@@ -1281,7 +1281,7 @@ def _disjoint(t):
 class KVCache:
     """K/V rows of `B` batch entries, `H` heads, up to `cap` tokens of `D` elements: k, v [B, H, cap, D] and - in the 8-bit formats
     "e4m3" / "int8" (codes; uint8 tensors or views of the type itself) - their fp32 scales ks, vs [B, H, cap]; value = code * scale.
-    "bf16" / "f32" hold the values.  Views with other strides are fine as long as D is contiguous (and the tokens of the scales are), k and v
+    "bf16" / "f32" hold the values.  Codes have to be finite (e4m3 has two that are not; kv_append writes neither).  Views with other strides are fine as long as D is contiguous (and the tokens of the scales are), k and v
     have the same strides, and the strides are multiples of 8 elements.  The cache does not know its lengths: the caller passes them."""
 
     def __init__(self, k, v, ks=None, vs=None, fmt="e4m3"):
@@ -1524,7 +1524,8 @@ def verify_draft(target, ids, draft=None, uniforms=None):
     [B, n + 1] in [0, 1)): draft i is accepted while u_i q_i(x_i) < p_i(x_i), with the draft model's probabilities `draft` fp32 [B, n, V]
     (None: the drafts were picked, q_i(x_i) = 1); the token after the accepted ones is drawn with the last uniform from the normalised
     max(p - q, 0) at a rejected draft, from p behind the last accepted one.  An id outside 0 .. V - 1 ends a row's drafts.  n = 0: plain sampling.
-    Greedy (uniforms = None; target may be logits): accepted while the id is the arg max (lowest index of ties).
+    Greedy (uniforms = None; target may be logits): accepted while the id is the arg max (lowest index of ties; unlike torch's, it ranks a NaN
+    below everything: a row without a number above -inf gives 0).
     -> (accepted int32 [B], token int64 [B])."""
     sig = (_sig(target), _sig(ids), _sig(draft), _sig(uniforms), torch._C._cuda_getDevice())
     hit = _SIGNATURES.get(sig)

@@ -1281,8 +1281,9 @@ def _disjoint(t):
 class KVCache:
     """K/V rows of `B` batch entries, `H` heads, up to `cap` tokens of `D` elements: k, v [B, H, cap, D] and - in the 8-bit formats
     "e4m3" / "int8" (codes; uint8 tensors or views of the type itself) - their fp32 scales ks, vs [B, H, cap]; value = code * scale.
-    "bf16" / "f32" hold the values.  Codes have to be finite (e4m3 has two that are not; kv_append writes neither).  Views with other strides are fine as long as D is contiguous (and the tokens of the scales are), k and v
-    have the same strides, and the strides are multiples of 8 elements.  The cache does not know its lengths: the caller passes them."""
+    "bf16" / "f32" hold the values.  Codes have to be finite (e4m3 has two that are not; kv_append writes neither).  Views with other strides
+    are fine as long as D is contiguous (and the tokens of the scales are), k and v have the same strides, and the strides are multiples of 8
+    elements.  The cache does not know its lengths: the caller passes them."""
 
     def __init__(self, k, v, ks=None, vs=None, fmt="e4m3"):
         _need(fmt in KV_FORMATS, f"KVCache: unknown format {fmt!r} (one of {sorted(KV_FORMATS)})")
@@ -1372,7 +1373,7 @@ def kv_append(cache, k, v, start=0):
     int32 [B] on the device), quantised to the cache's format.  Rows that fall outside the capacity are dropped.  No backward: tensors that
     require a gradient are refused while gradients are recorded (here and in the other two)."""
     if torch.is_grad_enabled():
-        _no_history("kv_append", k, v, cache.k, cache.v)
+        _no_history("kv_append", k, v, cache.k, cache.v, cache.ks, cache.vs)
     r = _kv_rows("kv_append", cache, start, k, v, False)
     if r:
         L.check(L.lib().smx_kv_append(C.byref(r[0]), r[1], _stream()), "smx_kv_append")
@@ -1381,7 +1382,7 @@ def kv_append(cache, k, v, start=0):
 def kv_read(cache, start, k, v):
     """The cache's values at positions start .. start + T - 1 into k, v [B, T, H, D] (fp32 / bf16).  Rows outside the capacity are left alone."""
     if torch.is_grad_enabled():
-        _no_history("kv_read", k, v, cache.k, cache.v)
+        _no_history("kv_read", k, v, cache.k, cache.v, cache.ks, cache.vs)
     r = _kv_rows("kv_read", cache, start, k, v, True)
     if r:
         L.check(L.lib().smx_kv_read(C.byref(r[0]), r[1], _stream()), "smx_kv_read")
